@@ -120,6 +120,75 @@ int rst_softmax_forward(rst_engine* engine, const double* x, double* out, size_t
 int rst_softmax_backward(rst_engine* engine, const double* grad, const double* output,
                          double* grad_input, size_t rows, size_t cols);
 
+/* ---- the residual block: layer norm, dropout, activations, Linear with activation and residual -
+ *      (no counterpart in the reference; x + Dropout(Linear(act(Linear(LayerNorm(x))))) and its
+ *      backward pass).  Parameter gradients are divided by the number of rows, as Linear's are
+ *      (src/module/linear.rs:62-66), and overwritten, never accumulated.  Arrays need their 8-byte
+ *      alignment only and have any extents.  Nothing here allocates or waits; launches recorded into
+ *      a graph of the caller's use the engine's scratch as the eager ones do: graphs of one engine run
+ *      one at a time, on its stream ------------------------------------------------------------------ */
+/* RST_ACT_GELU: z (1 + erf(z / sqrt 2)) / 2;  RST_ACT_GELU_TANH: z (1 + tanh(sqrt(2 / pi) (z +
+ * 0.044715 z^3))) / 2;  RST_ACT_SILU: z / (1 + exp(-z)).  At an infinite z all of them take their
+ * limit (value 0 or z, derivative 0 or 1); NaN stays NaN, but RST_ACT_RELU takes it to 0, with derivative
+ * 0, as rst_relu_forward does. */
+enum { RST_ACT_NONE = 0, RST_ACT_RELU = 1, RST_ACT_GELU = 2, RST_ACT_GELU_TANH = 3, RST_ACT_SILU = 4 };
+
+/* Each row r of x[rows,cols]: out = (x - m) rstd * weight + bias with m = mean(x), rstd = 1 / sqrt(
+ * mean((x - m)^2) + eps), eps >= 0.  weight, bias [1,cols]: NULL for ones / zeros.  mean, rstd [rows]
+ * receive what the backward pass needs; NULL: not kept (inference).  out may be x itself. */
+int rst_layer_norm_forward(rst_engine* engine, const double* x, const double* weight,
+                           const double* bias, double* out, double* mean, double* rstd, size_t rows,
+                           size_t cols, double eps);
+/* x, weight: the forward pass's; mean, rstd: what it kept.  With xh = (x - mean) rstd and u = grad *
+ * weight:  grad_input = rstd (u - mean(u) - xh mean(u xh)) + residual_grad  (residual_grad[rows,cols]:
+ * the gradient that reaches x past the layer; NULL: none),  grad_weight = colsum(grad * xh) / rows,
+ * grad_bias = colsum(grad) / rows  (NULL: skipped).  grad_input may be grad, x or residual_grad itself. */
+int rst_layer_norm_backward(rst_engine* engine, const double* grad, const double* x,
+                            const double* weight, const double* mean, const double* rstd,
+                            const double* residual_grad, double* grad_input, double* grad_weight,
+                            double* grad_bias, size_t rows, size_t cols);
+
+/* out[i] = (value(seed, stream, i) >= p ? x[i] / (1 - p) : 0) + residual[i], 0 <= p < 1, with value as
+ * in rst_fill_uniform(0, 1): a pure function, so no mask is stored and the backward pass draws the same
+ * numbers again from the same (seed, stream).  x[i] / (1 - p) is computed as x[i] times the rounded
+ * reciprocal.  A dropped element is 0 even where x is infinite or NaN.  residual NULL: nothing is added.
+ * out may be x or residual itself.  The numbers are arguments: a recorded graph replays the mask it was
+ * recorded with. */
+int rst_dropout_forward(rst_engine* engine, const double* x, const double* residual, double* out,
+                        size_t count, double p, uint64_t seed, uint64_t stream);
+/* out[i] = value(seed, stream, i) >= p ? grad[i] / (1 - p) : 0  (the residual's gradient is grad). */
+int rst_dropout_backward(rst_engine* engine, const double* grad, double* out, size_t count, double p,
+                         uint64_t seed, uint64_t stream);
+
+/* out = act(x) + residual;  out = grad * act'(pre) + residual, pre being what act was applied to (not
+ * read with RST_ACT_NONE).  residual NULL: nothing is added.  out may be an input. */
+int rst_activation_forward(rst_engine* engine, const double* x, const double* residual, double* out,
+                           size_t count, int activation);
+int rst_activation_backward(rst_engine* engine, const double* grad, const double* pre,
+                            const double* residual, double* out, size_t count, int activation);
+
+/* z = x[batch,in] . weight[out,in]^T + bias[1,out];  out[batch,out] = act(z) + residual[batch,out].
+ * bias, residual: NULL for none.  pre_out[batch,out] receives z for the backward pass (NULL: not kept).
+ * out and pre_out are no operand of the call. */
+int rst_linear_act_forward(rst_engine* engine, const double* x, const double* weight,
+                           const double* bias, const double* residual, double* pre_out, double* out,
+                           size_t batch, size_t in_features, size_t out_features, int activation);
+/* grad[batch,out] is the gradient with respect to the forward pass's out (the residual's gradient is
+ * grad itself).  dz = grad * act'(pre), kept in grad_pre[batch,out] (RST_ACT_NONE: dz = grad, pre and
+ * grad_pre are not used; otherwise both are needed and grad_pre may be grad or pre itself).
+ * grad_weight = dz^T . x / batch;  grad_bias = colsum(dz) / batch (NULL: skipped);
+ * grad_input[batch,in] = (dz . weight) * act_in'(input_pre) + residual_grad (NULL: skipped), where
+ * input_activation is what produced x from input_pre[batch,in] (its backward pass, fused as
+ * rst_linear_backward fuses ReLU's; RST_ACT_NONE: input_pre is not used) and residual_grad[batch,in],
+ * NULL for none, is what reaches this layer's input past it.  With both, residual_grad is the gradient
+ * with respect to input_pre.  The results are no operands of the call. */
+int rst_linear_act_backward(rst_engine* engine, const double* grad, const double* pre, int activation,
+                            double* grad_pre, const double* x, const double* weight,
+                            double* grad_weight, double* grad_bias, double* grad_input,
+                            const double* input_pre, int input_activation,
+                            const double* residual_grad, size_t batch, size_t in_features,
+                            size_t out_features);
+
 /* ---- CrossEntropyLoss (src/loss/cross_entropy.rs:34-47) ---------------------------------- */
 /* One pass: prob = softmax(pred); loss = -(sum truth*ln(prob)) / rows; grad_out = prob - truth
  * (what `backward()` returns; NOT divided by rows).  prob_out may be NULL.  host_loss may be

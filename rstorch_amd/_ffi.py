@@ -21,6 +21,7 @@ RST_ERR_OUT_OF_MEMORY = 6
 RST_ERR_UNSUPPORTED = 7
 
 LAYER_IDENTITY, LAYER_LINEAR, LAYER_RELU = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = 0, 1, 2, 3, 4
 
 KERNEL_NAMES = {
     0: "linear_forward", 1: "grad_weight", 2: "grad_bias", 3: "grad_input", 4: "relu_forward",
@@ -83,6 +84,14 @@ SIGNATURES = {
     "rst_softmax_rows": [_vp, _dp, _dp, _sz, _sz],
     "rst_softmax_forward": [_vp, _dp, _dp, _sz, _sz, _i32],
     "rst_softmax_backward": [_vp, _dp, _dp, _dp, _sz, _sz],
+    "rst_layer_norm_forward": [_vp, _dp, _dp, _dp, _dp, _dp, _dp, _sz, _sz, _dbl],
+    "rst_layer_norm_backward": [_vp, _dp, _dp, _dp, _dp, _dp, _dp, _dp, _dp, _dp, _sz, _sz],
+    "rst_dropout_forward": [_vp, _dp, _dp, _dp, _sz, _dbl, _u64, _u64],
+    "rst_dropout_backward": [_vp, _dp, _dp, _sz, _dbl, _u64, _u64],
+    "rst_activation_forward": [_vp, _dp, _dp, _dp, _sz, _i32],
+    "rst_activation_backward": [_vp, _dp, _dp, _dp, _dp, _sz, _i32],
+    "rst_linear_act_forward": [_vp, _dp, _dp, _dp, _dp, _dp, _dp, _sz, _sz, _sz, _i32],
+    "rst_linear_act_backward": [_vp, _dp, _dp, _i32, _dp, _dp, _dp, _dp, _dp, _dp, _dp, _i32, _dp, _sz, _sz, _sz],
     "rst_cross_entropy": [_vp, _dp, _dp, _dp, _dp, _sz, _sz, c_double_p],
     "rst_cross_entropy_accuracy": [_vp, _dp, _dp, _dp, _sz, _sz, c_double_p, c_double_p],
     "rst_cross_entropy_static": [_vp, _dp, _dp, _dp, _sz, _sz, c_double_p],

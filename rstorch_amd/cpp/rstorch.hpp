@@ -15,6 +15,10 @@
 // through parameters() or keeping the returned input gradient runs it on its own first.  Everything a
 // caller can observe is what the layer-by-layer path computes.  push / insert / remove drop the
 // compiled form.
+//
+// Beside the reference's layers stand those of a residual block: LayerNorm, Dropout, GELU, SiLU and
+// Residual.  A Sequential that holds one runs layer by layer, and a Linear takes the activation behind
+// it, a residual and, in the backward pass, the activation in front of it into its own launches.
 #pragma once
 
 #include <cmath>
@@ -334,6 +338,7 @@ class ReLU : public Module {
   void absorb_forward(const Array2& activation) { prev_input_ = activation; has_ = true; }
   void absorb_backward() { (void)take(); }
   bool has_cache() const { return has_; }
+  const Array2& cache() const { return prev_input_; }
 
  private:
   Array2 take() {
@@ -343,6 +348,163 @@ class ReLU : public Module {
   }
   Array2 prev_input_;
   bool has_ = false;
+};
+
+// ---- the residual block's element-wise layers ----------------------------------------------------
+namespace detail {
+inline const double* data_or_null(const Array2* a) { return a ? a->data() : nullptr; }
+// x + residual
+inline Array2 add(const Array2& x, const Array2& residual) {
+  if (!x.same_shape(residual)) throw Panic(RST_ERR_SHAPE, "residual shape");
+  Array2 out(x.nrows(), x.ncols(), x.engine_ref());
+  check(rst_activation_forward(x.engine(), x.data(), residual.data(), out.data(), x.size(), RST_ACT_NONE));
+  return out;
+}
+}  // namespace detail
+
+// An activation that a neighbouring Linear can take into its launches; keeps what it was applied to.
+class Activation : public Module {
+ public:
+  explicit Activation(int kind) : kind_(kind) {}
+  Array2 forward(Array2 input) override {
+    Array2 out(input.nrows(), input.ncols(), input.engine_ref());
+    check(rst_activation_forward(input.engine(), input.data(), nullptr, out.data(), input.size(), kind_));
+    absorb_forward(std::move(input));
+    return out;
+  }
+  Array2 backward(Array2 gradient) override {
+    if (!has_) throw Panic(RST_ERR_STATE, debug() + "::backward without a forward");
+    if (!pre_.same_shape(gradient)) throw Panic(RST_ERR_SHAPE, debug() + ": gradient shape");
+    Array2 pre = take();
+    Array2 out(pre.nrows(), pre.ncols(), pre.engine_ref());
+    check(rst_activation_backward(pre.engine(), gradient.data(), pre.data(), nullptr, out.data(), pre.size(), kind_));
+    return out;
+  }
+  Parameters parameters() override { return Parameters(); }
+  int kind() const { return kind_; }
+  // Sequential's fusion: the neighbouring Linear did this layer's work.
+  void absorb_forward(Array2 pre) { pre_ = std::move(pre); has_ = true; }
+  bool has_cache() const { return has_; }
+  Array2 take() {
+    has_ = false;
+    return std::move(pre_);
+  }
+
+ private:
+  int kind_;
+  Array2 pre_;
+  bool has_ = false;
+};
+
+class GELU : public Activation {
+ public:
+  explicit GELU(bool approximate = false) : Activation(approximate ? RST_ACT_GELU_TANH : RST_ACT_GELU) {}
+  std::string debug() const override { return kind() == RST_ACT_GELU ? "GELU" : "GELU { approximate: true }"; }
+};
+
+class SiLU : public Activation {
+ public:
+  SiLU() : Activation(RST_ACT_SILU) {}
+  std::string debug() const override { return "SiLU"; }
+};
+
+// Training (the state it starts in): each element is zero with probability p, the others are scaled by
+// 1 / (1 - p); evaluation: the input.  Call number n of the module draws value(seed, n, index) of the
+// library's generator, and backward draws it again; no mask is stored.
+class Dropout : public Module {
+ public:
+  explicit Dropout(double p) : Dropout(p, fresh_seed()) {}
+  Dropout(double p, uint64_t seed) : p_(p), seed_(seed) {
+    if (!(p >= 0.0 && p < 1.0)) throw Panic(RST_ERR_INVALID_ARGUMENT, "Dropout: p is not in [0, 1)");
+  }
+  Array2 forward(Array2 input) override { return forward_impl(std::move(input), nullptr); }
+  Array2 forward_impl(Array2 input, const Array2* residual) {
+    if (residual && !residual->same_shape(input)) throw Panic(RST_ERR_SHAPE, "residual shape");
+    rows_ = input.nrows();
+    cols_ = input.ncols();
+    has_ = true;
+    drawn_ = training_ && p_ > 0.0;
+    if (!drawn_) return residual ? detail::add(input, *residual) : input;
+    stream_ = calls_++;
+    Array2 out(rows_, cols_, input.engine_ref());
+    check(rst_dropout_forward(input.engine(), input.data(), detail::data_or_null(residual), out.data(), input.size(),
+                              p_, seed_, stream_));
+    return out;
+  }
+  Array2 backward(Array2 gradient) override {
+    if (!has_) throw Panic(RST_ERR_STATE, "Dropout::backward without a forward");
+    if (gradient.nrows() != rows_ || gradient.ncols() != cols_) throw Panic(RST_ERR_SHAPE, "Dropout: gradient shape");
+    has_ = false;
+    if (!drawn_) return gradient;
+    Array2 out(rows_, cols_, gradient.engine_ref());
+    check(rst_dropout_backward(gradient.engine(), gradient.data(), out.data(), gradient.size(), p_, seed_, stream_));
+    return out;
+  }
+  Parameters parameters() override { return Parameters(); }
+  void train() override { training_ = true; }
+  void eval() override { training_ = false; }
+  std::string debug() const override { return "Dropout { p: " + std::to_string(p_) + " }"; }
+
+ private:
+  double p_;
+  uint64_t seed_, calls_ = 0, stream_ = 0;
+  size_t rows_ = 0, cols_ = 0;
+  bool training_ = true, has_ = false, drawn_ = false;
+};
+
+// Each row to mean 0 and variance 1, then times weight plus bias (1, size), which start as ones and
+// zeros; their gradients are divided by the number of rows, as Linear's are.
+class LayerNorm : public Module {
+ public:
+  explicit LayerNorm(size_t size, double eps = 1e-5)
+      : size_(size), eps_(eps), weight_(Array2::full(1, size, 1.0).mark_rewritten_in_place()),
+        bias_(Array2::zeros(1, size).mark_rewritten_in_place()) {}
+  Array2 forward(Array2 input) override {
+    if (input.ncols() != size_) throw Panic(RST_ERR_SHAPE, "LayerNorm: input width");
+    Array2 out(input.nrows(), size_), mean(input.nrows(), 1), rstd(input.nrows(), 1);
+    check(rst_layer_norm_forward(input.engine(), input.data(), weight_.data(), bias_.data(), out.data(), mean.data(),
+                                 rstd.data(), input.nrows(), size_, eps_));
+    x_ = std::move(input);
+    mean_ = std::move(mean);
+    rstd_ = std::move(rstd);
+    has_ = true;
+    return out;
+  }
+  Array2 backward(Array2 gradient) override { return backward_impl(std::move(gradient), nullptr); }
+  Array2 backward_impl(Array2 gradient, const Array2* residual) {
+    if (!has_) throw Panic(RST_ERR_STATE, "LayerNorm::backward without a forward");
+    if (!gradient.same_shape(x_) || (residual && !residual->same_shape(x_)))
+      throw Panic(RST_ERR_SHAPE, "LayerNorm: gradient shape");
+    has_ = false;
+    Array2 x = std::move(x_), mean = std::move(mean_), rstd = std::move(rstd_);
+    if (grad_weight_.empty_handle()) {
+      grad_weight_ = Array2(1, size_).mark_rewritten_in_place();
+      grad_bias_ = Array2(1, size_).mark_rewritten_in_place();
+    }
+    Array2 gx(x.nrows(), size_);
+    check(rst_layer_norm_backward(x.engine(), gradient.data(), x.data(), weight_.data(), mean.data(), rstd.data(),
+                                  detail::data_or_null(residual), gx.data(), grad_weight_.data(), grad_bias_.data(),
+                                  x.nrows(), size_));
+    has_grad_ = true;
+    return gx;
+  }
+  Parameters parameters() override {
+    if (!has_grad_) throw Panic(RST_ERR_STATE, "LayerNorm::parameters before any backward");
+    Parameters p;
+    p.add(weight_, grad_weight_).add(bias_, grad_bias_);
+    return p;
+  }
+  std::string debug() const override { return "LayerNorm(" + std::to_string(size_) + ")"; }
+  Array2& weight() { return weight_; }
+  Array2& bias() { return bias_; }
+  Array2& grad_weight() { return grad_weight_; }
+  Array2& grad_bias() { return grad_bias_; }
+
+ private:
+  size_t size_;
+  double eps_;
+  Array2 weight_, bias_, grad_weight_, grad_bias_, x_, mean_, rstd_;
+  bool has_ = false, has_grad_ = false;
 };
 
 // ---- Softmax: src/module/activation/softmax.rs:5-78 ---------------------------------------------
@@ -417,6 +579,39 @@ class Linear : public Module {
     check(rst_linear_backward(x.engine(), gradient.data(), x.data(), weight_.data(), grad_weight_.data(),
                               grad_bias_.data(), gx.data(), mask_by_input ? x.data() : nullptr, x.nrows(),
                               in_, out_));
+    return gx;
+  }
+  // The same with an activation behind the layer, a residual, an activation in front of it.
+  // *pre (with an activation): what the activation was applied to.
+  Array2 forward_act(Array2 input, int activation, const Array2* residual, Array2* pre) {
+    if (input.ncols() != in_) throw Panic(RST_ERR_SHAPE, "Linear: input width");
+    Array2 out(input.nrows(), out_);
+    if (residual && !residual->same_shape(out)) throw Panic(RST_ERR_SHAPE, "residual shape");
+    if (pre) *pre = Array2(input.nrows(), out_);
+    check(rst_linear_act_forward(input.engine(), input.data(), weight_.data(), bias_.data(),
+                                 detail::data_or_null(residual), pre ? pre->data() : nullptr, out.data(),
+                                 input.nrows(), in_, out_, activation));
+    prev_input_ = std::move(input);
+    has_input_ = true;
+    return out;
+  }
+  Array2 backward_act(Array2 gradient, const Array2* input_pre, int input_activation, const Array2* residual) {
+    if (!has_input_) throw Panic(RST_ERR_STATE, "Linear::backward without a forward");
+    if (gradient.nrows() != prev_input_.nrows() || gradient.ncols() != out_) throw Panic(RST_ERR_SHAPE, "Linear: gradient shape");
+    if ((input_pre && !input_pre->same_shape(prev_input_)) || (residual && !residual->same_shape(prev_input_)))
+      throw Panic(RST_ERR_SHAPE, "Linear: shape of the activation in front or of the residual's gradient");
+    has_input_ = false;
+    Array2 x = std::move(prev_input_);
+    if (!has_grad_) {
+      grad_weight_ = Array2(out_, in_).mark_rewritten_in_place();
+      grad_bias_ = Array2(1, out_).mark_rewritten_in_place();
+      has_grad_ = true;
+    }
+    Array2 gx(x.nrows(), in_);
+    check(rst_linear_act_backward(x.engine(), gradient.data(), nullptr, RST_ACT_NONE, nullptr, x.data(),
+                                  weight_.data(), grad_weight_.data(), grad_bias_.data(), gx.data(),
+                                  detail::data_or_null(input_pre), input_activation, detail::data_or_null(residual),
+                                  x.nrows(), in_, out_));
     return gx;
   }
   Parameters parameters() override {
@@ -671,44 +866,107 @@ class Sequential : public Module {
 
   Array2 forward(Array2 input) override {
     if (detail::Plan* plan = compiled()) return plan->forward(std::move(input));
+    return layers_forward(std::move(input), nullptr);
+  }
+  // Layer by layer; residual (or NULL) is added to the result, by the last layer where it can.
+  Array2 layers_forward(Array2 input, const Array2* residual) {
+    drop_plan();
     const int n = int(layers_.size());
+    const int last = prev_real(n);  // (-1: nothing but Identity)
     for (int i = 0; i < n; ++i) {
       Module* l = layers_[i].get();
       if (l->layer_kind() == RST_LAYER_LINEAR) {
+        auto* linear = static_cast<Linear*>(l);
         int j = next_real(i);
-        if (j >= 0 && layers_[j]->layer_kind() == RST_LAYER_RELU) {
-          input = static_cast<Linear*>(l)->forward_impl(std::move(input), true);
-          static_cast<ReLU*>(layers_[j].get())->absorb_forward(input);
-          // Identity layers between the two pass the handle through; the ReLU is done
+        Module* behind = j >= 0 ? layers_[j].get() : nullptr;
+        const bool relu = behind && behind->layer_kind() == RST_LAYER_RELU;
+        auto* act = dynamic_cast<Activation*>(behind);
+        const Array2* added = j == last ? residual : nullptr;
+        if (act || relu) {
+          if (relu && !added) {
+            input = linear->forward_impl(std::move(input), true);
+            static_cast<ReLU*>(behind)->absorb_forward(input);
+          } else {
+            Array2 pre;
+            input = linear->forward_act(std::move(input), act ? act->kind() : RST_ACT_RELU, added, &pre);
+            if (act) act->absorb_forward(std::move(pre));
+            else static_cast<ReLU*>(behind)->absorb_forward(pre);
+          }
+          if (added) residual = nullptr;
+          // Identity layers between the two pass the handle through; the activation is done
           for (int k = i + 1; k < j; ++k) input = layers_[k]->forward(std::move(input));
           i = j;
+          continue;
+        }
+        if (residual && i == last) {
+          input = linear->forward_act(std::move(input), RST_ACT_NONE, residual, nullptr);
+          residual = nullptr;
+          continue;
+        }
+      }
+      if (residual && i == last) {
+        if (auto* dropout = dynamic_cast<Dropout*>(l)) {
+          input = dropout->forward_impl(std::move(input), residual);
+          residual = nullptr;
           continue;
         }
       }
       input = l->forward(std::move(input));
     }
-    return input;
+    return residual ? detail::add(input, *residual) : input;
   }
 
   Array2 backward(Array2 gradient) override {
     if (plan_ && plan_->valid_for(layers_)) return plan_->backward(std::move(gradient));
+    return layers_backward(std::move(gradient), nullptr);
+  }
+  // Layer by layer; residual (or NULL) is added to the input gradient, by the first layer where it can.
+  Array2 layers_backward(Array2 gradient, const Array2* residual) {
     const int n = int(layers_.size());
+    const int first = next_real(-1);
     for (int i = n - 1; i >= 0; --i) {
       Module* l = layers_[i].get();
       if (l->layer_kind() == RST_LAYER_LINEAR) {
+        auto* linear = static_cast<Linear*>(l);
         int j = prev_real(i);
-        if (j >= 0 && layers_[j]->layer_kind() == RST_LAYER_RELU &&
-            static_cast<ReLU*>(layers_[j].get())->has_cache()) {
-          gradient = static_cast<Linear*>(l)->backward_impl(std::move(gradient), true);
-          static_cast<ReLU*>(layers_[j].get())->absorb_backward();
+        Module* before = j >= 0 ? layers_[j].get() : nullptr;
+        auto* relu = before && before->layer_kind() == RST_LAYER_RELU ? static_cast<ReLU*>(before) : nullptr;
+        if (relu && !relu->has_cache()) relu = nullptr;
+        auto* act = dynamic_cast<Activation*>(before);
+        if (act && !act->has_cache()) act = nullptr;
+        const Array2* added = j == first ? residual : nullptr;
+        if (act || relu) {
+          if (relu && !added) {
+            gradient = linear->backward_impl(std::move(gradient), true);
+            relu->absorb_backward();
+          } else if (relu) {
+            gradient = linear->backward_act(std::move(gradient), &relu->cache(), RST_ACT_RELU, added);
+            relu->absorb_backward();
+          } else {
+            Array2 pre = act->take();
+            gradient = linear->backward_act(std::move(gradient), &pre, act->kind(), added);
+          }
+          if (added) residual = nullptr;
           for (int k = i - 1; k > j; --k) gradient = layers_[k]->backward(std::move(gradient));
           i = j;
+          continue;
+        }
+        if (residual && i == first) {
+          gradient = linear->backward_act(std::move(gradient), nullptr, RST_ACT_NONE, residual);
+          residual = nullptr;
+          continue;
+        }
+      }
+      if (residual && i == first) {
+        if (auto* norm = dynamic_cast<LayerNorm*>(l)) {
+          gradient = norm->backward_impl(std::move(gradient), residual);
+          residual = nullptr;
           continue;
         }
       }
       gradient = l->backward(std::move(gradient));
     }
-    return gradient;
+    return residual ? detail::add(gradient, *residual) : gradient;
   }
   void train() override { for (auto& l : layers_) l->train(); }
   void eval() override { for (auto& l : layers_) l->eval(); }
@@ -764,6 +1022,39 @@ class Sequential : public Module {
     return -1;
   }
   std::vector<std::unique_ptr<Module>> layers_;
+};
+
+// x + inner(x): layers whose output has the shape of their input.  The addition (and, in the backward
+// pass, that of the gradient that passes the layers by) is done by the inner layers' own launches where
+// the last one is a Linear, an activation behind a Linear, or Dropout, and the first one a Linear or
+// LayerNorm.
+class Residual : public Module {
+ public:
+  explicit Residual(Sequential inner) : inner_(std::move(inner)) {}
+  Array2 forward(Array2 input) override {
+    const Array2 x = input;
+    Array2 out = inner_.layers_forward(std::move(input), &x);
+    rows_ = x.nrows();
+    cols_ = x.ncols();
+    has_ = true;
+    return out;
+  }
+  Array2 backward(Array2 gradient) override {
+    if (!has_) throw Panic(RST_ERR_STATE, "Residual::backward without a forward");
+    if (gradient.nrows() != rows_ || gradient.ncols() != cols_) throw Panic(RST_ERR_SHAPE, "Residual: gradient shape");
+    has_ = false;
+    const Array2 g = gradient;
+    return inner_.layers_backward(std::move(gradient), &g);
+  }
+  Parameters parameters() override { return inner_.parameters(); }
+  void train() override { inner_.train(); }
+  void eval() override { inner_.eval(); }
+  std::string debug() const override { return "Residual(" + inner_.debug() + ")"; }
+
+ private:
+  Sequential inner_;
+  size_t rows_ = 0, cols_ = 0;
+  bool has_ = false;
 };
 
 // sequential!(...): src/module/sequential.rs:62-74

@@ -183,6 +183,22 @@ int launch_accuracy(hipStream_t s, const double* pred, const double* truth, size
                     size_t cols, unsigned long long* hits, unsigned long long* hits_mirror = nullptr,
                     bool* mirrored = nullptr, ResultSlot* slots = nullptr, unsigned ticket = 0);
 
+// ---- residual block: activations, dropout, layer norm ------------------------------------------
+// out = act(z) [+ residual] / out = g * act'(z) [+ residual] (RST_ACT_*; residual NULL: none; with
+// RST_ACT_NONE the second does not read z).  out may be any of the inputs.
+int launch_act_forward(hipStream_t s, int activation, const double* z, const double* residual, double* out, size_t n);
+int launch_act_backward(hipStream_t s, int activation, const double* g, const double* z, const double* residual,
+                        double* out, size_t n);
+int launch_dropout(hipStream_t s, const double* x, const double* residual, double* out, size_t n, double p,
+                   uint64_t seed, uint64_t stream);
+int launch_layer_norm_forward(hipStream_t s, const double* x, const double* w, const double* b, double* out,
+                              double* mean, double* rstd, size_t rows, size_t cols, double eps);
+// workspace: scratch for the column sums of the workgroups
+int launch_layer_norm_backward(hipStream_t s, const double* grad, const double* x, const double* weight,
+                               const double* mean, const double* rstd, const double* residual, double* grad_input,
+                               double* grad_weight, double* grad_bias, size_t rows, size_t cols, double* workspace,
+                               size_t workspace_count);
+
 int launch_fill_uniform(hipStream_t s, double* dst, size_t n, uint64_t seed, uint64_t stream,
                         double lo, double hi);
 int launch_fill_normal(hipStream_t s, double* dst, size_t n, uint64_t seed, uint64_t stream,

@@ -19,8 +19,10 @@ into its parameter arena (the layers keep views) and from then on
   it on its own first, so every value a caller can observe is the value the reference computes at
   that point.  The input gradient itself is only computed if the returned array is kept.
 
-Any other layer list (a ``Softmax`` module, a user-defined ``Module``) runs layer by layer.  Changing
-the layer list (``push`` / ``insert`` / ``remove``) drops the compiled form; it is rebuilt on the next
+Any other layer list (a ``Softmax`` module, the residual block's ``LayerNorm`` / ``Dropout`` / ``GELU`` /
+``SiLU`` / ``Residual``, a user-defined ``Module``) runs layer by layer; a ``Linear`` takes the activation
+behind it, a residual and, in the backward pass, the activation in front of it into its own launches.
+Changing the layer list (``push`` / ``insert`` / ``remove``) drops the compiled form; it is rebuilt on the next
 ``forward``.
 """
 import ctypes
@@ -28,7 +30,7 @@ import weakref
 
 from . import _ffi
 from .engine import Array2, as_array2, default_engine
-from .init import InitParameters, KaimingNormal
+from .init import InitParameters, KaimingNormal, _fresh_seed
 
 
 class Parameter:
@@ -136,6 +138,195 @@ class ReLU(Module):
         return "ReLU"
 
 
+def _same_shape(residual, shape):
+    if residual is not None and residual.shape != shape:
+        raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "residual %r vs %r" % (residual.shape, shape))
+
+
+def _add(x, residual):
+    """x + residual in a new array."""
+    _same_shape(residual, x.shape)
+    out = x.engine.empty(x.rows, x.cols)
+    _ffi.check(x.engine.lib.rst_activation_forward(x.engine.handle, x.ptr, residual.ptr, out.ptr, x.size,
+                                                   _ffi.ACT_NONE))
+    return out
+
+
+class _Activation(Module):
+    """An element-wise activation of the residual block: keeps what it was applied to."""
+
+    kind = None
+
+    def __init__(self):
+        self.prev_input = None
+
+    @classmethod
+    def new(cls):
+        return cls()
+
+    def forward(self, input):
+        x = as_array2(input)
+        out = x.engine.empty(x.rows, x.cols)
+        _ffi.check(x.engine.lib.rst_activation_forward(x.engine.handle, x.ptr, None, out.ptr, x.size, self.kind))
+        self.prev_input = x
+        return out
+
+    def backward(self, gradient):
+        if self.prev_input is None:
+            raise _ffi.StateError(_ffi.RST_ERR_STATE, "%r.backward without a forward" % self)
+        g = as_array2(gradient, self.prev_input.engine)
+        if g.shape != self.prev_input.shape:
+            raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "gradient %r vs input %r" % (g.shape, self.prev_input.shape))
+        x, self.prev_input = self.prev_input, None
+        out = x.engine.empty(x.rows, x.cols)
+        _ffi.check(x.engine.lib.rst_activation_backward(x.engine.handle, g.ptr, x.ptr, None, out.ptr, x.size,
+                                                        self.kind))
+        return out
+
+    # used by Sequential when the neighbouring Linear kernels do this layer's work
+    def _absorb_forward(self, pre):
+        self.prev_input = pre
+
+    def _absorb_backward(self):
+        self.prev_input = None
+
+    def __repr__(self):
+        return type(self).__name__
+
+
+class GELU(_Activation):
+    """x P(x), P the normal distribution's integral; ``approximate``: its tanh form."""
+
+    def __init__(self, approximate=False):
+        super().__init__()
+        self.kind = _ffi.ACT_GELU_TANH if approximate else _ffi.ACT_GELU
+
+    def __repr__(self):
+        return "GELU(approximate=True)" if self.kind == _ffi.ACT_GELU_TANH else "GELU"
+
+
+class SiLU(_Activation):
+    """x / (1 + exp(-x))."""
+
+    kind = _ffi.ACT_SILU
+
+
+class Dropout(Module):
+    """In training (the state a module starts in; ``train`` / ``eval`` switch) zeroes each element with
+    probability ``p`` and scales the others by 1 / (1 - p); in evaluation hands its input through.  No
+    mask is stored: call number n of the module draws value(seed, n, index) of the library's generator,
+    and ``backward`` draws it again."""
+
+    def __init__(self, p=0.5, seed=None):
+        if not 0.0 <= p < 1.0:
+            raise ValueError("p = %r is not in [0, 1)" % (p,))
+        self.p, self.seed = float(p), _fresh_seed() if seed is None else int(seed) & 0xFFFFFFFFFFFFFFFF
+        self.training = True
+        self._calls = 0
+        self._kept = None  # (shape, stream) of the last forward; stream None: handed through
+
+    @classmethod
+    def new(cls, p):
+        return cls(p)
+
+    def train(self):
+        self.training = True
+
+    def eval(self):
+        self.training = False
+
+    def _forward(self, input, residual):
+        x = as_array2(input)
+        _same_shape(residual, x.shape)
+        if not self.training or self.p == 0.0:
+            self._kept = (x.shape, None)
+            return x if residual is None else _add(x, residual)
+        stream, self._calls = self._calls, self._calls + 1
+        out = x.engine.empty(x.rows, x.cols)
+        _ffi.check(x.engine.lib.rst_dropout_forward(x.engine.handle, x.ptr, residual.ptr if residual else None,
+                                                    out.ptr, x.size, self.p, self.seed, stream))
+        self._kept = (x.shape, stream)
+        return out
+
+    def forward(self, input):
+        return self._forward(input, None)
+
+    def backward(self, gradient):
+        if self._kept is None:
+            raise _ffi.StateError(_ffi.RST_ERR_STATE, "Dropout.backward without a forward")
+        g = as_array2(gradient)
+        shape, stream = self._kept
+        if g.shape != shape:
+            raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "gradient %r vs input %r" % (g.shape, shape))
+        self._kept = None
+        if stream is None:
+            return g
+        out = g.engine.empty(g.rows, g.cols)
+        _ffi.check(g.engine.lib.rst_dropout_backward(g.engine.handle, g.ptr, out.ptr, g.size, self.p, self.seed,
+                                                     stream))
+        return out
+
+    def __repr__(self):
+        return "Dropout(%g)" % self.p
+
+
+class LayerNorm(Module):
+    """Each row to mean 0 and variance 1 (over its ``size`` columns, ``eps`` added to the variance), then
+    times ``weight`` plus ``bias`` (1, size), which start as ones and zeros.  Their gradients are divided
+    by the number of rows, as Linear's are."""
+
+    def __init__(self, size, eps=1e-5, engine=None):
+        eng = engine or default_engine()
+        self.engine, self.size, self.eps = eng, int(size), float(eps)
+        self.weight, self.bias = eng.full(1, self.size, 1.0), eng.zeros(1, self.size)
+        self.grad_weight = self.grad_bias = None
+        self._kept = None  # (x, mean, rstd) of the last forward
+
+    @classmethod
+    def new(cls, size):
+        return cls(size)
+
+    def forward(self, input):
+        x = as_array2(input, self.engine)
+        if x.cols != self.size:
+            raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "input has %d features, layer expects %d" % (x.cols, self.size))
+        out, mean, rstd = (self.engine.empty(x.rows, n) for n in (x.cols, 1, 1))
+        _ffi.check(self.engine.lib.rst_layer_norm_forward(
+            self.engine.handle, x.ptr, self.weight.ptr, self.bias.ptr, out.ptr, mean.ptr, rstd.ptr, x.rows, x.cols,
+            self.eps))
+        self._kept = (x, mean, rstd)
+        return out
+
+    def _backward(self, gradient, residual):
+        if self._kept is None:
+            raise _ffi.StateError(_ffi.RST_ERR_STATE, "LayerNorm.backward without a forward")
+        g = as_array2(gradient, self.engine)
+        x, mean, rstd = self._kept
+        if g.shape != x.shape:
+            raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "gradient %r vs input %r" % (g.shape, x.shape))
+        _same_shape(residual, x.shape)
+        self._kept = None
+        grad_weight = self.grad_weight or self.engine.empty(1, self.size)
+        grad_bias = self.grad_bias or self.engine.empty(1, self.size)
+        gx = self.engine.empty(x.rows, x.cols)
+        _ffi.check(self.engine.lib.rst_layer_norm_backward(
+            self.engine.handle, g.ptr, x.ptr, self.weight.ptr, mean.ptr, rstd.ptr, residual.ptr if residual else None,
+            gx.ptr, grad_weight.ptr, grad_bias.ptr, x.rows, x.cols))
+        self.grad_weight, self.grad_bias = grad_weight, grad_bias
+        return gx
+
+    def backward(self, gradient):
+        return self._backward(gradient, None)
+
+    def parameters(self):
+        if self.grad_weight is None:
+            raise _ffi.StateError(_ffi.RST_ERR_STATE, "LayerNorm.parameters before any backward (no gradient yet)")
+        return Parameters().add(self.weight, self.grad_weight).add(self.bias, self.grad_bias)
+
+    def __repr__(self):
+        return "LayerNorm(%d)" % self.size
+
+
 class Softmax(Module):
     """src/module/activation/softmax.rs:5-78: softmax along an axis; the backward pass builds the
     reference's single batch-summed Jacobian."""
@@ -241,6 +432,46 @@ class Linear(Module):
 
     def backward(self, gradient):
         return self._backward(gradient, False)
+
+    # The same with an activation behind the layer, a residual, an activation in front of it.
+    def _forward_act(self, input, activation, residual):
+        """(act(z) + residual, z) in one pass; z only with an activation."""
+        x = as_array2(input, self.engine)
+        if x.cols != self.input_size:
+            raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "input has %d features, layer expects %d"
+                                  % (x.cols, self.input_size))
+        _same_shape(residual, (x.rows, self.output_size))
+        out = self.engine.empty(x.rows, self.output_size)
+        pre = self.engine.empty(x.rows, self.output_size) if activation != _ffi.ACT_NONE else None
+        _ffi.check(self.engine.lib.rst_linear_act_forward(
+            self.engine.handle, x.ptr, self.weight.ptr, self.bias.ptr, residual.ptr if residual else None,
+            pre.ptr if pre else None, out.ptr, x.rows, self.input_size, self.output_size, activation))
+        self.prev_input = x
+        return out, pre
+
+    def _backward_act(self, gradient, input_pre, input_activation, residual):
+        if self.prev_input is None:
+            raise _ffi.StateError(_ffi.RST_ERR_STATE, "Linear.backward without a forward")
+        g = as_array2(gradient, self.engine)
+        x = self.prev_input
+        if g.shape != (x.rows, self.output_size):
+            raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "gradient %r vs expected %r"
+                                  % (g.shape, (x.rows, self.output_size)))
+        _same_shape(residual, x.shape)
+        if input_pre is not None and input_pre.shape != x.shape:
+            raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "the activation in front saw %r, this layer %r"
+                                  % (input_pre.shape, x.shape))
+        self.prev_input = None
+        if self.grad_weight is None:
+            self.grad_weight = self.engine.empty(self.output_size, self.input_size)
+            self.grad_bias = self.engine.empty(1, self.output_size)
+        self._has_grad = True
+        gx = self.engine.empty(x.rows, self.input_size)
+        _ffi.check(self.engine.lib.rst_linear_act_backward(
+            self.engine.handle, g.ptr, None, _ffi.ACT_NONE, None, x.ptr, self.weight.ptr, self.grad_weight.ptr,
+            self.grad_bias.ptr, gx.ptr, input_pre.ptr if input_pre else None, input_activation,
+            residual.ptr if residual else None, x.rows, self.input_size, self.output_size))
+        return gx
 
     def parameters(self):
         if not self._has_grad:
@@ -454,6 +685,15 @@ class Sequential(Module):
         self._drop_plan()
         return self.layers.pop(index)
 
+    def _output_size(self, width):
+        """Columns of what the layers return for an input of ``width`` columns."""
+        for layer in self.layers:
+            if type(layer) is Linear:
+                width = layer.output_size
+            elif isinstance(layer, Sequential):
+                width = layer._output_size(width)
+        return width
+
     def _next_real(self, i):
         for j in range(i + 1, len(self.layers)):
             if not isinstance(self.layers[j], Identity):
@@ -470,25 +710,51 @@ class Sequential(Module):
         plan = self._compiled()
         if plan is not None:
             return plan.forward(input)
+        return self._layers_forward(input, None)
+
+    def _layers_forward(self, input, residual):
+        """Layer by layer; residual (or None) is added to the result, by the last layer where it can."""
         x = input
+        last = self._prev_real(len(self.layers))  # (-1: nothing but Identity)
         skip = set()
         for i, layer in enumerate(self.layers):
             if i in skip:
                 continue
             if type(layer) is Linear:
                 j = self._next_real(i)
-                if j >= 0 and type(self.layers[j]) is ReLU:
+                behind = self.layers[j] if j >= 0 else None
+                if type(behind) is ReLU and (residual is None or j != last):
                     x = layer._forward(x, True)
-                    self.layers[j]._absorb_forward(x)
+                    behind._absorb_forward(x)
                     skip.add(j)
                     continue
+                if isinstance(behind, _Activation) or type(behind) is ReLU:
+                    kind = behind.kind if isinstance(behind, _Activation) else _ffi.ACT_RELU
+                    x, pre = layer._forward_act(x, kind, residual if j == last else None)
+                    behind._absorb_forward(pre)
+                    skip.add(j)
+                    residual = None if j == last else residual
+                    continue
+                if residual is not None and i == last:
+                    x, _ = layer._forward_act(x, _ffi.ACT_NONE, residual)
+                    residual = None
+                    continue
+            if residual is not None and i == last and type(layer) is Dropout:
+                x = layer._forward(x, residual)
+                residual = None
+                continue
             x = layer.forward(x)
-        return x
+        return x if residual is None else _add(as_array2(x), residual)
 
     def backward(self, gradient):
         if self._plan is not None and self._plan.valid_for(self.layers):
             return self._plan.backward(gradient)
+        return self._layers_backward(gradient, None)
+
+    def _layers_backward(self, gradient, residual):
+        """Layer by layer; residual (or None) is added to the input gradient, by the first layer where it can."""
         g = gradient
+        first = self._next_real(-1)
         skip = set()
         for i in range(len(self.layers) - 1, -1, -1):
             if i in skip:
@@ -496,14 +762,29 @@ class Sequential(Module):
             layer = self.layers[i]
             if type(layer) is Linear:
                 j = self._prev_real(i)
-                if j >= 0 and type(self.layers[j]) is ReLU and \
-                        self.layers[j].prev_input is not None:
+                before = self.layers[j] if j >= 0 else None
+                if type(before) is ReLU and before.prev_input is not None and (residual is None or j != first):
                     g = layer._backward(g, True)
-                    self.layers[j]._absorb_backward()
+                    before._absorb_backward()
                     skip.add(j)
                     continue
+                if (isinstance(before, _Activation) or type(before) is ReLU) and before.prev_input is not None:
+                    kind = before.kind if isinstance(before, _Activation) else _ffi.ACT_RELU
+                    g = layer._backward_act(g, before.prev_input, kind, residual if j == first else None)
+                    before._absorb_backward()
+                    skip.add(j)
+                    residual = None if j == first else residual
+                    continue
+                if residual is not None and i == first:
+                    g = layer._backward_act(g, None, _ffi.ACT_NONE, residual)
+                    residual = None
+                    continue
+            if residual is not None and i == first and type(layer) is LayerNorm:
+                g = layer._backward(g, residual)
+                residual = None
+                continue
             g = layer.backward(g)
-        return g
+        return g if residual is None else _add(as_array2(g), residual)
 
     def train(self):
         for layer in self.layers:
@@ -522,6 +803,56 @@ class Sequential(Module):
 
     def __repr__(self):
         return "Sequential(%s)" % ", ".join(repr(l) for l in self.layers)
+
+
+class Residual(Module):
+    """x + inner(x); ``inner``: a layer or a list of layers whose output has the shape of its input.  The
+    addition (and, in the backward pass, that of the gradient that passes the layers by) is done by the
+    inner layers' own launches where the last one is a Linear, an activation behind a Linear, or Dropout, and
+    the first one a Linear or LayerNorm."""
+
+    def __init__(self, inner):
+        if isinstance(inner, Sequential):
+            self.inner = inner
+        else:
+            self.inner = Sequential(list(inner) if isinstance(inner, (list, tuple)) else [inner])
+        self._shape = None
+
+    @classmethod
+    def new(cls, inner):
+        return cls(inner)
+
+    def forward(self, input):
+        x = as_array2(input)
+        self.inner._drop_plan()  # (a compiled form would add in a pass of its own)
+        wide = self.inner._output_size(x.cols)
+        if wide != x.cols:
+            raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "a residual of %d features around layers that return %d"
+                                  % (x.cols, wide))
+        out = self.inner._layers_forward(x, x)
+        self._shape = x.shape
+        return out
+
+    def backward(self, gradient):
+        if self._shape is None:
+            raise _ffi.StateError(_ffi.RST_ERR_STATE, "Residual.backward without a forward")
+        g = as_array2(gradient)
+        if g.shape != self._shape:
+            raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "gradient %r vs input %r" % (g.shape, self._shape))
+        self._shape = None
+        return self.inner._layers_backward(g, g)
+
+    def parameters(self):
+        return self.inner.parameters()
+
+    def train(self):
+        self.inner.train()
+
+    def eval(self):
+        self.inner.eval()
+
+    def __repr__(self):
+        return "Residual(%s)" % ", ".join(repr(l) for l in self.inner.layers)
 
 
 def sequential(*layers):

@@ -172,6 +172,7 @@ extern "C" hipError_t __hipPopCallConfiguration(dim3* g, dim3* b, size_t* shmem,
 }
 hipError_t hipLaunchKernel(const void*, dim3 g, dim3 b, void**, size_t, hipStream_t) {
   if (g.x == 0 || g.y == 0 || g.z == 0 || b.x == 0 || b.x * b.y * b.z > 1024) die("launch with an empty or oversized grid/block", nullptr);
+  if ((unsigned long long)g.x * b.x >= 1ull << 32 || g.y > 65535 || g.z > 65535) die("launch with a grid beyond the runtime's limits", nullptr);
   if (g_capturing) ++g_captured_nodes; else ++g_launches;
   return hipSuccess;
 }
