@@ -169,19 +169,19 @@ int rst_activation_backward(rst_engine* engine, const double* grad, const double
 
 /* z = x[batch,in] . weight[out,in]^T + bias[1,out];  out[batch,out] = act(z) + residual[batch,out].
  * bias, residual: NULL for none.  pre_out[batch,out] receives z for the backward pass (NULL: not kept).
- * out and pre_out are no operand of the call. */
+ * out may be residual itself; out and pre_out are no other operand. */
 int rst_linear_act_forward(rst_engine* engine, const double* x, const double* weight,
                            const double* bias, const double* residual, double* pre_out, double* out,
                            size_t batch, size_t in_features, size_t out_features, int activation);
 /* grad[batch,out] is the gradient with respect to the forward pass's out (the residual's gradient is
  * grad itself).  dz = grad * act'(pre), kept in grad_pre[batch,out] (RST_ACT_NONE: dz = grad, pre and
- * grad_pre are not used; otherwise both are needed and grad_pre may be grad or pre itself).
+ * grad_pre are not used; otherwise both are needed, and grad_pre may be grad or pre itself).
  * grad_weight = dz^T . x / batch;  grad_bias = colsum(dz) / batch (NULL: skipped);
  * grad_input[batch,in] = (dz . weight) * act_in'(input_pre) + residual_grad (NULL: skipped), where
  * input_activation is what produced x from input_pre[batch,in] (its backward pass, fused as
  * rst_linear_backward fuses ReLU's; RST_ACT_NONE: input_pre is not used) and residual_grad[batch,in],
  * NULL for none, is what reaches this layer's input past it.  With both, residual_grad is the gradient
- * with respect to input_pre.  The results are no operands of the call. */
+ * with respect to input_pre.  grad_input may be input_pre or residual_grad itself. */
 int rst_linear_act_backward(rst_engine* engine, const double* grad, const double* pre, int activation,
                             double* grad_pre, const double* x, const double* weight,
                             double* grad_weight, double* grad_bias, double* grad_input,

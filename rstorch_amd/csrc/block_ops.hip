@@ -100,17 +100,17 @@ int rst_linear_act_forward(rst_engine* e, const double* x, const double* weight,
   RST_TRY(check_dim("linear_act_forward", batch, "batch"));
   RST_TRY(check_dim("linear_act_forward", in_features, "in_features"));
   RST_TRY(check_dim("linear_act_forward", out_features, "out_features"));
+  const ActEpilogue act{activation, nullptr, residual, pre_out};
   GemmDesc d{};
-  d.A = x; d.B = weight; d.C = pre_out ? pre_out : out;
+  d.A = x; d.B = weight; d.C = out;
   d.M = (int)batch; d.N = (int)out_features; d.K = (int)in_features;
   d.lda = (long)in_features; d.ldb = (long)in_features; d.ldc = (long)out_features;
   d.a_kc = true; d.b_kc = true;
   d.bias = bias;
   d.epilogue = bias ? EPI_BIAS : EPI_NONE;
   d.workspace = e->d_gemm_ws; d.workspace_count = e->gemm_ws_count;
-  RST_TRY(launch_gemm(e->stream, d));
-  if (activation == RST_ACT_NONE && !residual && !pre_out) return RST_OK;
-  return launch_act_forward(e->stream, activation, d.C, residual, out, batch * out_features);
+  if (activation != RST_ACT_NONE || residual || pre_out) d.act = &act;
+  return launch_gemm(e->stream, d);
 }
 
 int rst_linear_act_backward(rst_engine* e, const double* grad, const double* pre, int activation, double* grad_pre,
@@ -136,11 +136,10 @@ int rst_linear_act_backward(rst_engine* e, const double* grad, const double* pre
     RST_TRY(launch_act_backward(e->stream, activation, grad, pre, nullptr, grad_pre, batch * out_features));
     grad = grad_pre;
   }
-  RST_TRY(rst_linear_backward(e, grad, x, weight, grad_weight, grad_bias, grad_input, nullptr, batch, in_features,
-                              out_features));
-  if (!grad_input || (input_activation == RST_ACT_NONE && !residual_grad)) return RST_OK;
-  return launch_act_backward(e->stream, input_activation, grad_input, input_pre, residual_grad, grad_input,
-                             batch * in_features);
+  const ActEpilogue act{input_activation, input_pre, residual_grad, nullptr};
+  const bool plain = input_activation == RST_ACT_NONE && !residual_grad;
+  return engine_linear_backward(e, grad, x, weight, grad_weight, grad_bias, grad_input, nullptr, plain ? nullptr : &act,
+                                batch, in_features, out_features);
 }
 
 }  // extern "C"

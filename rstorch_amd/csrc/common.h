@@ -69,6 +69,17 @@ struct GemmDesc {
   // scratch for split-K partial products (small outputs with a long contraction); NULL: never split
   double* workspace;
   size_t workspace_count;
+  // the residual block's epilogue instead of `epilogue` (layouts with A contraction-contiguous), or NULL
+  const struct ActEpilogue* act;
+};
+
+// Every array is [M][N] with C's leading dimension.  B contraction-contiguous (forward): z = acc + bias,
+// pre = z, C = act(z) + residual.  B output-contiguous (input gradient): C = acc * act'(source) + residual.
+struct ActEpilogue {
+  int activation;          // RST_ACT_*
+  const double* source;    // input gradient with an activation: what it was applied to
+  const double* residual;  // or NULL; may be C itself, as source may be
+  double* pre;             // forward: receives z, or NULL
 };
 
 int launch_gemm(hipStream_t stream, const GemmDesc& d);
@@ -83,7 +94,8 @@ int launch_gemm_pair(hipStream_t stream, const GemmDesc& input_grad, const GemmD
 // sliced ones; same results as launch_gemm on each, except that from a batch of about 4096 a
 // group of weight gradients runs as K-sliced 128x128 tiles whose slices differ from a lone launch's
 // (equal within rounding, 1e-13).  The descriptors share one workspace, of which the group as a
-// whole takes gemm_group_workspace(d, count) doubles.
+// whole takes gemm_group_workspace(d, count) doubles.  A member with an ActEpilogue: a weight gradient and the
+// layer's input gradient, which carries it.
 bool can_group_gemm(const GemmDesc& d);
 size_t gemm_group_workspace(const GemmDesc* d, int count);
 int max_gemm_group();
@@ -273,6 +285,11 @@ int engine_cross_entropy(rst_engine* e, double* row_loss, const double* pred, co
 // `ahead` (launches the caller wants on the stream before the host waits), waits
 int engine_accuracy(rst_engine* e, const double* pred, const double* truth, size_t rows, size_t cols,
                     int (*ahead)(void*) = nullptr, void* ahead_arg = nullptr);
+// the three products of Linear::backward; input_act (or NULL): the input gradient's epilogue
+int engine_linear_backward(rst_engine* e, const double* grad, const double* x, const double* weight,
+                           double* grad_weight, double* grad_bias, double* grad_input,
+                           const double* relu_mask_source, const ActEpilogue* input_act, size_t batch,
+                           size_t in_features, size_t out_features);
 // the fused classifier head (launch_head_ce) with the engine's loss words, mirror and ticket
 int engine_head_cross_entropy(rst_engine* e, double* row_loss, const double* h, const double* w,
                               const double* bias, const double* truth, double* logits, double* grad,

@@ -340,6 +340,7 @@ struct GemmLaunch {
   const GemmParams* p2;     // the second problem of a pair
   int first_blocks;         // workgroups of the first problem of a pair
   const GemmGroup* group;   // the members of a grouped launch
+  bool act;                 // the residual block's epilogue: one more array or two, indexed as C
 };
 #ifdef RST_GEMM_LAUNCH_OBSERVER
 void observe_gemm_launch(const GemmLaunch& launch);

@@ -24,6 +24,7 @@
 #include <cstdlib>
 #include <type_traits>
 
+#include "activation.h"
 #include "common.h"
 #include "gemm_addressing.h"
 
@@ -244,11 +245,114 @@ __device__ __forceinline__ void store_block_interior(const GemmParams& p, const 
   }
 }
 
+// What a finished block becomes: the epilogue the launch asks for.
+struct PlainFinish {
+  template <int TM, int TN>
+  __device__ __forceinline__ void store(const GemmParams& p, const v4d* acc, int row0, int col0, int lr, int lk,
+                                        bool interior) const {
+    // (a true division keeps to the general path: its temporaries on top of a batch of parameter
+    // loads do not fit the registers that the accumulators leave)
+    if (interior && (p.epilogue != EPI_DIVIDE || p.divisor_reciprocal != 0.0)) {
+      switch (p.epilogue) {
+        case EPI_BIAS: store_block_interior<TM, TN, EPI_BIAS, false, false>(p, acc, p.C, p.ldc, row0, col0, lr, lk); break;
+        case EPI_BIAS_RELU: store_block_interior<TM, TN, EPI_BIAS_RELU, false, false>(p, acc, p.C, p.ldc, row0, col0, lr, lk); break;
+        case EPI_RELU: store_block_interior<TM, TN, EPI_RELU, false, false>(p, acc, p.C, p.ldc, row0, col0, lr, lk); break;
+        case EPI_MASK: store_block_interior<TM, TN, EPI_MASK, false, false>(p, acc, p.C, p.ldc, row0, col0, lr, lk); break;
+        case EPI_DIVIDE:
+          if (p.sgd_parm) store_block_interior<TM, TN, EPI_DIVIDE, true, true>(p, acc, p.C, p.ldc, row0, col0, lr, lk);
+          else store_block_interior<TM, TN, EPI_DIVIDE, false, true>(p, acc, p.C, p.ldc, row0, col0, lr, lk);
+          break;
+        default: store_block_interior<TM, TN, EPI_NONE, false, false>(p, acc, p.C, p.ldc, row0, col0, lr, lk); break;
+      }
+      return;
+    }
+    switch (p.epilogue) {
+      case EPI_BIAS: store_block<TM, TN, EPI_BIAS, false>(p, acc, row0, col0, lr, lk); break;
+      case EPI_BIAS_RELU: store_block<TM, TN, EPI_BIAS_RELU, false>(p, acc, row0, col0, lr, lk); break;
+      case EPI_RELU: store_block<TM, TN, EPI_RELU, false>(p, acc, row0, col0, lr, lk); break;
+      case EPI_MASK: store_block<TM, TN, EPI_MASK, false>(p, acc, row0, col0, lr, lk); break;
+      case EPI_DIVIDE:
+        if (p.sgd_parm) store_block<TM, TN, EPI_DIVIDE, true>(p, acc, row0, col0, lr, lk);
+        else store_block<TM, TN, EPI_DIVIDE, false>(p, acc, row0, col0, lr, lk);
+        break;
+      default: store_block<TM, TN, EPI_NONE, false>(p, acc, row0, col0, lr, lk); break;
+    }
+  }
+};
+
+// The residual block's epilogue (ActEpilogue): what an element needs from memory is requested for a fragment
+// row at a time, from clamped addresses, and only the stores are predicated (as in store_block).
+template <int TM, int TN, int ACT, bool GRAD>
+__device__ __forceinline__ void store_block_act(const GemmParams& p, const ActEpilogue& e, const v4d* acc, int row0,
+                                                int col0, int lr, int lk) {
+  constexpr bool SOURCE = GRAD && ACT != RST_ACT_NONE;
+  double bias[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int col = acc_col(col0, j, lr);
+    bias[j] = !GRAD && p.bias ? p.bias[col < p.N ? col : p.N - 1] : 0.0;
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    double source[TN][4], residual[TN][4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = acc_row(row0, i, r, lk);
+      const size_t base = (size_t)(row < p.M ? row : p.M - 1) * p.ldc;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int col = acc_col(col0, j, lr);
+        const size_t at = base + (col < p.N ? col : p.N - 1);
+        if (SOURCE) source[j][r] = e.source[at];
+        residual[j][r] = e.residual ? e.residual[at] : 0.0;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = acc_row(row0, i, r, lk);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int col = acc_col(col0, j, lr);
+        double v = acc[i * TN + j][r];
+        if (row < p.M && col < p.N) {
+          const size_t at = (size_t)row * p.ldc + col;
+          if (GRAD) {
+            if (ACT != RST_ACT_NONE) v *= act_gradient<ACT>(source[j][r]);
+          } else {
+            if (p.bias) v += bias[j];
+            if (e.pre) e.pre[at] = v;
+            v = act_value<ACT>(v);
+          }
+          if (e.residual) v += residual[j][r];
+          p.C[at] = v;
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // one fragment row at a time: the live registers of two would spill
+  }
+}
+
+template <bool GRAD>
+struct ActFinish {
+  const ActEpilogue& e;
+  template <int TM, int TN>
+  __device__ __forceinline__ void store(const GemmParams& p, const v4d* acc, int row0, int col0, int lr, int lk,
+                                        bool) const {
+    switch (e.activation) {
+      case RST_ACT_RELU: store_block_act<TM, TN, RST_ACT_RELU, GRAD>(p, e, acc, row0, col0, lr, lk); break;
+      case RST_ACT_GELU: store_block_act<TM, TN, RST_ACT_GELU, GRAD>(p, e, acc, row0, col0, lr, lk); break;
+      case RST_ACT_GELU_TANH: store_block_act<TM, TN, RST_ACT_GELU_TANH, GRAD>(p, e, acc, row0, col0, lr, lk); break;
+      case RST_ACT_SILU: store_block_act<TM, TN, RST_ACT_SILU, GRAD>(p, e, acc, row0, col0, lr, lk); break;
+      default: store_block_act<TM, TN, RST_ACT_NONE, GRAD>(p, e, acc, row0, col0, lr, lk); break;
+    }
+  }
+};
+
 // Writes the block either as raw partial products of K slice `split` (the reduction applies the
 // epilogue later) or finished, with the epilogue the launch asks for.
-template <int TM, int TN>
-__device__ __forceinline__ void write_block(const GemmParams& p, const v4d* acc, int row0, int col0,
-                                            int lr, int lk, int split) {
+template <int TM, int TN, class Finish>
+__device__ __forceinline__ void write_block(const GemmParams& p, const Finish& finish, const v4d* acc, int row0,
+                                            int col0, int lr, int lk, int split) {
   // the block origin is the same for the whole wavefront: keep it in scalar registers
   row0 = __builtin_amdgcn_readfirstlane(row0);
   col0 = __builtin_amdgcn_readfirstlane(col0);
@@ -273,33 +377,7 @@ __device__ __forceinline__ void write_block(const GemmParams& p, const v4d* acc,
       }
     return;
   }
-  // (a true division keeps to the general path: its temporaries on top of a batch of parameter
-  // loads do not fit the registers that the accumulators leave)
-  if (interior && (p.epilogue != EPI_DIVIDE || p.divisor_reciprocal != 0.0)) {
-    switch (p.epilogue) {
-      case EPI_BIAS: store_block_interior<TM, TN, EPI_BIAS, false, false>(p, acc, p.C, p.ldc, row0, col0, lr, lk); break;
-      case EPI_BIAS_RELU: store_block_interior<TM, TN, EPI_BIAS_RELU, false, false>(p, acc, p.C, p.ldc, row0, col0, lr, lk); break;
-      case EPI_RELU: store_block_interior<TM, TN, EPI_RELU, false, false>(p, acc, p.C, p.ldc, row0, col0, lr, lk); break;
-      case EPI_MASK: store_block_interior<TM, TN, EPI_MASK, false, false>(p, acc, p.C, p.ldc, row0, col0, lr, lk); break;
-      case EPI_DIVIDE:
-        if (p.sgd_parm) store_block_interior<TM, TN, EPI_DIVIDE, true, true>(p, acc, p.C, p.ldc, row0, col0, lr, lk);
-        else store_block_interior<TM, TN, EPI_DIVIDE, false, true>(p, acc, p.C, p.ldc, row0, col0, lr, lk);
-        break;
-      default: store_block_interior<TM, TN, EPI_NONE, false, false>(p, acc, p.C, p.ldc, row0, col0, lr, lk); break;
-    }
-    return;
-  }
-  switch (p.epilogue) {
-    case EPI_BIAS: store_block<TM, TN, EPI_BIAS, false>(p, acc, row0, col0, lr, lk); break;
-    case EPI_BIAS_RELU: store_block<TM, TN, EPI_BIAS_RELU, false>(p, acc, row0, col0, lr, lk); break;
-    case EPI_RELU: store_block<TM, TN, EPI_RELU, false>(p, acc, row0, col0, lr, lk); break;
-    case EPI_MASK: store_block<TM, TN, EPI_MASK, false>(p, acc, row0, col0, lr, lk); break;
-    case EPI_DIVIDE:
-      if (p.sgd_parm) store_block<TM, TN, EPI_DIVIDE, true>(p, acc, row0, col0, lr, lk);
-      else store_block<TM, TN, EPI_DIVIDE, false>(p, acc, row0, col0, lr, lk);
-      break;
-    default: store_block<TM, TN, EPI_NONE, false>(p, acc, row0, col0, lr, lk); break;
-  }
+  finish.template store<TM, TN>(p, acc, row0, col0, lr, lk, interior);
 }
 
 // Bias gradient inside the weight-gradient contraction (output-contiguous A = grad^T): the
@@ -344,9 +422,9 @@ __device__ __forceinline__ void colsum_finish(double partial, double* __restrict
 // in K order, so a short contraction pays one trip to memory instead of one per step.  The
 // accumulation order, and with it every bit of the result, is the same either way.
 // lds_a / lds_b: room for kStages tiles of the respective operand (tile_lds_doubles).
-template <int BM, int BN, int WGM, int WGN, bool A_KC, bool B_KC, bool VEC, int BURST = 0>
+template <int BM, int BN, int WGM, int WGN, bool A_KC, bool B_KC, bool VEC, int BURST = 0, class Finish = PlainFinish>
 __device__ __forceinline__ void gemm_tile(const GemmParams& p, const int block, double* __restrict__ lds_a_base,
-                                          double* __restrict__ lds_b_base) {
+                                          double* __restrict__ lds_b_base, const Finish& finish = Finish()) {
   constexpr int kThreads = WGM * WGN * 64;
   using GA = TileGeom<BM, A_KC, kThreads>;
   using GB = TileGeom<BN, B_KC, kThreads>;
@@ -457,7 +535,7 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, const int block, 
     if (do_colsum) colsum_finish<BM, kThreads>(colsum_partial, lds_b(0), tid, m0, split, p);
   }
 
-  write_block<TM, TN>(p, &acc[0][0], m0 + wm * WM, n0 + wn * WN, lr, lk, split);
+  write_block<TM, TN>(p, finish, &acc[0][0], m0 + wm * WM, n0 + wn * WN, lr, lk, split);
 }
 
 // LDS doubles that gemm_tile needs for one operand
@@ -594,9 +672,9 @@ constexpr int kDmaStage = BK * (128 + 16);  // the larger of the two tile layout
 // output (wave-uniform tests around the MFMAs).  For grids of few tiles around narrow outputs - a
 // 100 x 784 weight gradient - where the fragments beyond the edge are a fifth of the work; the
 // large products leave it off and keep their instruction stream free of branches.
-template <bool A_KC, bool B_KC, int WGM, int WGN, int STAGES, int DIST, bool RAGGED = false>
+template <bool A_KC, bool B_KC, int WGM, int WGN, int STAGES, int DIST, bool RAGGED = false, class Finish = PlainFinish>
 __device__ __forceinline__ void dma_tile(const GemmParams& p, int block, double* __restrict__ lds_a,
-                                         double* __restrict__ lds_b) {
+                                         double* __restrict__ lds_b, const Finish& finish = Finish()) {
   constexpr int BM = 128, BN = 128, NW = WGM * WGN;
   constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   constexpr int CH = 16 / NW;  // 1 KiB chunks of each operand tile moved by one wavefront
@@ -817,7 +895,7 @@ __device__ __forceinline__ void dma_tile(const GemmParams& p, int block, double*
     if (do_colsum) colsum_finish<BM, NW * 64>(colsum_partial, lds_b, tid, m0, split, p);
   }
 
-  write_block<TM, TN>(p, &acc[0][0], m0 + wm * WM, n0 + wn * WN, lr, lk, split);
+  write_block<TM, TN>(p, finish, &acc[0][0], m0 + wm * WM, n0 + wn * WN, lr, lk, split);
 }
 
 template <bool A_KC, bool B_KC, int WGM, int WGN, int STAGES, int DIST>
@@ -891,13 +969,12 @@ __device__ __forceinline__ v2d read_pair64(uint32_t stage_bytes, int e, int pr) 
   }
 }
 
-template <bool B_KC>
-__global__ __launch_bounds__(256, 2) void gemm_f64_mfma_dma64(const GemmParams p) {
+// lds_a / lds_b: kT64Stages * kT64Stage doubles each
+template <bool B_KC, class Finish = PlainFinish>
+__device__ __forceinline__ void dma64_tile(const GemmParams& p, const int block, double* __restrict__ lds_a,
+                                           double* __restrict__ lds_b, const Finish& finish = Finish()) {
   constexpr bool A_KC = true;  // the forward and input-gradient layouts (where this kernel pays)
-  __shared__ __attribute__((aligned(1024))) double lds_a[kT64Stages * kT64Stage];
-  __shared__ __attribute__((aligned(1024))) double lds_b[kT64Stages * kT64Stage];
   constexpr int BM = kT64, BN = kT64, NW = 4, TM = 2, TN = 2, CH = 2;
-  const int block = (int)blockIdx.x;
   const TileCoord tc = tile_of_block(p.tiles_m, p.tiles_n, block);
   const int split = tc.split;  // K slice of this workgroup (0 without split-K)
   const int tile_m = tc.tile_m, tile_n = tc.tile_n;
@@ -1057,7 +1134,55 @@ __global__ __launch_bounds__(256, 2) void gemm_f64_mfma_dma64(const GemmParams p
   for (; kt + kT64Stages < nk; ++kt) tile(kt, std::true_type{});
   for (; kt < nk; ++kt) tile(kt, std::false_type{});
 #undef RST_FENCE
-  write_block<TM, TN>(p, &acc[0][0], m0 + wm * 32, n0 + wn * 32, lr, lk, split);
+  write_block<TM, TN>(p, finish, &acc[0][0], m0 + wm * 32, n0 + wn * 32, lr, lk, split);
+}
+
+template <bool B_KC>
+__global__ __launch_bounds__(256, 2) void gemm_f64_mfma_dma64(const GemmParams p) {
+  __shared__ __attribute__((aligned(1024))) double lds_a[kT64Stages * kT64Stage];
+  __shared__ __attribute__((aligned(1024))) double lds_b[kT64Stages * kT64Stage];
+  dma64_tile<B_KC>(p, (int)blockIdx.x, lds_a, lds_b);
+}
+
+// ---- the same tiles with the residual block's epilogue ------------------------------------------
+// (forward: B contraction-contiguous; input gradient: B output-contiguous)
+template <int BM, int BN, int WGM, int WGN, bool B_KC, bool VEC, int BURST>
+__global__ __launch_bounds__(WGM * WGN * 64, (BURST > 0 ? 1 : WGM * WGN >= 8 ? 4 : 2)) void gemm_f64_mfma_act(
+    const GemmParams p, const ActEpilogue e) {
+  __shared__ __attribute__((aligned(16))) double lds_a[tile_lds_doubles<BM, true, WGM * WGN * 64, BURST>()];
+  __shared__ __attribute__((aligned(16))) double lds_b[tile_lds_doubles<BN, B_KC, WGM * WGN * 64, BURST>()];
+  gemm_tile<BM, BN, WGM, WGN, true, B_KC, VEC, BURST>(p, (int)blockIdx.x, lds_a, lds_b, ActFinish<!B_KC>{e});
+}
+
+// A layer's weight gradient (member 0) and its input gradient with the epilogue (member 1) in one grid.
+template <int BURST>
+__global__ __launch_bounds__(256, (BURST > 0 ? 1 : 2)) void gemm_f64_mfma_grads_act(const GemmGroup g, const ActEpilogue e) {
+  __shared__ __attribute__((aligned(16))) double lds_a[tile_lds_doubles<32, false, 256, BURST>()];
+  __shared__ __attribute__((aligned(16))) double lds_b[tile_lds_doubles<32, false, 256, BURST>()];
+  const int i = group_member_of_block(g.first_block, g.count, (int)blockIdx.x);
+  const int block = (int)blockIdx.x - g.first_block[i];
+  const ActFinish<true> finish{e};
+  switch (2 * i + g.p[i].unaligned) {
+    case 0: gemm_tile<32, 32, 2, 2, false, false, true, BURST>(g.p[i], block, lds_a, lds_b); break;
+    case 1: gemm_tile<32, 32, 2, 2, false, false, false, BURST>(g.p[i], block, lds_a, lds_b); break;
+    case 2: gemm_tile<32, 32, 2, 2, true, false, true, BURST>(g.p[i], block, lds_a, lds_b, finish); break;
+    default: gemm_tile<32, 32, 2, 2, true, false, false, BURST>(g.p[i], block, lds_a, lds_b, finish); break;
+  }
+}
+
+template <bool B_KC>
+__global__ __launch_bounds__(512, 4) void gemm_f64_mfma_dma_act(const GemmParams p, const ActEpilogue e) {
+  constexpr int A_SIZE = 128 * BK, B_SIZE = B_KC ? 128 * BK : kDmaStage;
+  __shared__ __attribute__((aligned(1024))) double lds_a[2 * A_SIZE];
+  __shared__ __attribute__((aligned(1024))) double lds_b[2 * B_SIZE];
+  dma_tile<true, B_KC, 2, 4, 2, 1, false>(p, (int)blockIdx.x, lds_a, lds_b, ActFinish<!B_KC>{e});
+}
+
+template <bool B_KC>
+__global__ __launch_bounds__(256, 2) void gemm_f64_mfma_dma64_act(const GemmParams p, const ActEpilogue e) {
+  __shared__ __attribute__((aligned(1024))) double lds_a[kT64Stages * kT64Stage];
+  __shared__ __attribute__((aligned(1024))) double lds_b[kT64Stages * kT64Stage];
+  dma64_tile<B_KC>(p, (int)blockIdx.x, lds_a, lds_b, ActFinish<!B_KC>{e});
 }
 
 // Two independent products in one grid: workgroups [0, first_blocks) work on `first`, the others on
@@ -1152,8 +1277,62 @@ __global__ __launch_bounds__(256) void split_reduce_group_kernel(const GemmGroup
   split_reduce_body(g.p[i], (size_t)((int)blockIdx.x - g.first_reduce_block[i]));
 }
 
-int launch_split_reduce(hipStream_t stream, const GemmParams& p) {
+// ... with the residual block's epilogue
+template <bool GRAD>
+__device__ __forceinline__ void split_reduce_act_body(const GemmParams& p, const ActEpilogue& e, const size_t block) {
   const size_t mn = (size_t)p.M * p.N;
+  const size_t i = block * 256 + threadIdx.x;
+  if (i >= mn) return;
+  double v = ordered_slice_sum(p.ws + i, mn, p.split_k);
+  const int row = (int)(i / p.N), col = (int)(i - (size_t)row * p.N);
+  const size_t at = (size_t)row * p.ldc + col;
+  if (GRAD) {
+    const double z = e.activation != RST_ACT_NONE ? e.source[at] : 0.0;
+    switch (e.activation) {
+      case RST_ACT_RELU: v *= act_gradient<RST_ACT_RELU>(z); break;
+      case RST_ACT_GELU: v *= act_gradient<RST_ACT_GELU>(z); break;
+      case RST_ACT_GELU_TANH: v *= act_gradient<RST_ACT_GELU_TANH>(z); break;
+      case RST_ACT_SILU: v *= act_gradient<RST_ACT_SILU>(z); break;
+      default: break;
+    }
+  } else {
+    if (p.bias) v += p.bias[col];
+    if (e.pre) e.pre[at] = v;
+    switch (e.activation) {
+      case RST_ACT_RELU: v = act_value<RST_ACT_RELU>(v); break;
+      case RST_ACT_GELU: v = act_value<RST_ACT_GELU>(v); break;
+      case RST_ACT_GELU_TANH: v = act_value<RST_ACT_GELU_TANH>(v); break;
+      case RST_ACT_SILU: v = act_value<RST_ACT_SILU>(v); break;
+      default: break;
+    }
+  }
+  if (e.residual) v += e.residual[at];
+  p.C[at] = v;
+}
+
+template <bool GRAD>
+__global__ __launch_bounds__(256) void split_reduce_act_kernel(const GemmParams p, const ActEpilogue e) {
+  split_reduce_act_body<GRAD>(p, e, blockIdx.x);
+}
+
+// (of gemm_f64_mfma_grads_act)
+__global__ __launch_bounds__(256) void split_reduce_grads_act_kernel(const GemmGroup g, const ActEpilogue e) {
+  const int i = group_member_of_block(g.first_reduce_block, g.count, (int)blockIdx.x);
+  const size_t block = (size_t)((int)blockIdx.x - g.first_reduce_block[i]);
+  if (i == 1) split_reduce_act_body<true>(g.p[1], e, block);
+  else split_reduce_body(g.p[0], block);
+}
+
+// e: the residual block's epilogue of a product whose B is (GRAD: output-) contraction-contiguous, or NULL
+template <bool GRAD = false>
+int launch_split_reduce(hipStream_t stream, const GemmParams& p, const ActEpilogue* e = nullptr) {
+  const size_t mn = (size_t)p.M * p.N;
+  if (e) {
+    RST_OBSERVE_GEMM(GemmKernel::kSplitReduce, 0, 0, 0, 0, false, false, false, 0, (long long)((mn + 255) / 256), 256, &p, nullptr, 0, nullptr, true);
+    hipLaunchKernelGGL(split_reduce_act_kernel<GRAD>, dim3((unsigned)((mn + 255) / 256)), dim3(256), 0, stream, p, *e);
+    RST_HIP(hipGetLastError());
+    return RST_OK;
+  }
   RST_OBSERVE_GEMM(GemmKernel::kSplitReduce, 0, 0, 0, 0, false, false, false, 0, (long long)((mn + 255) / 256), 256, &p, nullptr, 0, nullptr);
   hipLaunchKernelGGL(split_reduce_kernel, dim3((unsigned)((mn + 255) / 256)), dim3(256), 0, stream, p);
   RST_HIP(hipGetLastError());
@@ -1175,7 +1354,7 @@ int compute_units() {
 
 // want_split > 1: cut K into that many slices (the caller has checked the workspace)
 template <bool A_KC, bool B_KC>
-int launch_dma(hipStream_t stream, GemmParams p, int want_split = 0) {
+int launch_dma(hipStream_t stream, GemmParams p, int want_split = 0, const ActEpilogue* e = nullptr) {
   p.tiles_m = (p.M + 127) / 128;
   p.tiles_n = (p.N + 127) / 128;
   p.split_k = 1;
@@ -1204,7 +1383,14 @@ int launch_dma(hipStream_t stream, GemmParams p, int want_split = 0) {
   // more than one round of workgroups (two per CU fit): stagger the first round by 0.4 us per K step
   p.first_round = 2 * compute_units();
   p.dephase_ticks = blocks > p.first_round ? (p.steps_per_split < 250 ? 40 * p.steps_per_split : 10000) : 0;
-  RST_OBSERVE_GEMM(GemmKernel::kDma128, 128, 128, 2, 4, A_KC, B_KC, p.unaligned == 0, 0, blocks, 512, &p, nullptr, 0, nullptr);
+  RST_OBSERVE_GEMM(GemmKernel::kDma128, 128, 128, 2, 4, A_KC, B_KC, p.unaligned == 0, 0, blocks, 512, &p, nullptr, 0, nullptr, e != nullptr);
+  if constexpr (A_KC) {
+    if (e) {
+      hipLaunchKernelGGL(gemm_f64_mfma_dma_act<B_KC>, dim3((unsigned)blocks), dim3(512), 0, stream, p, *e);
+      RST_HIP(hipGetLastError());
+      return p.split_k > 1 ? launch_split_reduce<!B_KC>(stream, p, e) : RST_OK;
+    }
+  }
   hipLaunchKernelGGL((gemm_f64_mfma_dma<A_KC, B_KC, 2, 4, 2, 1>), dim3((unsigned)blocks),
                      dim3(512), 0, stream, p);
   RST_HIP(hipGetLastError());
@@ -1214,7 +1400,7 @@ int launch_dma(hipStream_t stream, GemmParams p, int want_split = 0) {
 
 // 64x64 direct-to-LDS tiles, optionally on `slices` K slices (the caller has checked the workspace)
 template <bool B_KC>
-int launch_dma64(hipStream_t stream, GemmParams p, int slices) {
+int launch_dma64(hipStream_t stream, GemmParams p, int slices, const ActEpilogue* e = nullptr) {
   p.tiles_m = (p.M + kT64 - 1) / kT64;
   p.tiles_n = (p.N + kT64 - 1) / kT64;
   const int nk = dma_whole_steps(p.K, p.k_reserve);
@@ -1230,7 +1416,12 @@ int launch_dma64(hipStream_t stream, GemmParams p, int slices) {
     }
   }
   if (blocks > 0x7fffffffLL) return fail(RST_ERR_UNSUPPORTED, "contraction grid too large");
-  RST_OBSERVE_GEMM(GemmKernel::kDma64, 64, 64, 2, 2, true, B_KC, p.unaligned == 0, 0, blocks, 256, &p, nullptr, 0, nullptr);
+  RST_OBSERVE_GEMM(GemmKernel::kDma64, 64, 64, 2, 2, true, B_KC, p.unaligned == 0, 0, blocks, 256, &p, nullptr, 0, nullptr, e != nullptr);
+  if (e) {
+    hipLaunchKernelGGL(gemm_f64_mfma_dma64_act<B_KC>, dim3((unsigned)blocks), dim3(256), 0, stream, p, *e);
+    RST_HIP(hipGetLastError());
+    return p.split_k > 1 ? launch_split_reduce<!B_KC>(stream, p, e) : RST_OK;
+  }
   hipLaunchKernelGGL((gemm_f64_mfma_dma64<B_KC>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
   RST_HIP(hipGetLastError());
   if (p.split_k > 1) RST_TRY(launch_split_reduce(stream, p));
@@ -1271,7 +1462,8 @@ void plan_slices(GemmParams& p, long long blocks, long long split_below, long lo
 }
 
 template <int BM, int BN, int WGM, int WGN, bool A_KC, bool B_KC, bool VEC>
-int launch_one(hipStream_t stream, GemmParams p, long long split_below = 256, long long want_blocks = 2048) {
+int launch_one(hipStream_t stream, GemmParams p, long long split_below = 256, long long want_blocks = 2048,
+               const ActEpilogue* e = nullptr) {
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
   long long blocks = (long long)p.tiles_m * p.tiles_n;
@@ -1279,7 +1471,19 @@ int launch_one(hipStream_t stream, GemmParams p, long long split_below = 256, lo
   blocks *= p.split_k;
   if (blocks > 0x7fffffffLL) return fail(RST_ERR_UNSUPPORTED, "contraction grid too large");
   const bool burst = BM == 32 && BN == 32 && blocks <= compute_units();
-  RST_OBSERVE_GEMM(GemmKernel::kStaged, BM, BN, WGM, WGN, A_KC, B_KC, VEC, burst ? kBurst : 0, blocks, WGM * WGN * 64, &p, nullptr, 0, nullptr);
+  RST_OBSERVE_GEMM(GemmKernel::kStaged, BM, BN, WGM, WGN, A_KC, B_KC, VEC, burst ? kBurst : 0, blocks, WGM * WGN * 64, &p, nullptr, 0, nullptr, e != nullptr);
+  if constexpr (A_KC) {
+    if (e) {
+      if (burst)
+        hipLaunchKernelGGL((gemm_f64_mfma_act<BM, BN, WGM, WGN, B_KC, VEC, (BM == 32 ? kBurst : 0)>),
+                           dim3((unsigned)blocks), dim3(WGM * WGN * 64), 0, stream, p, *e);
+      else
+        hipLaunchKernelGGL((gemm_f64_mfma_act<BM, BN, WGM, WGN, B_KC, VEC, 0>), dim3((unsigned)blocks),
+                           dim3(WGM * WGN * 64), 0, stream, p, *e);
+      RST_HIP(hipGetLastError());
+      return p.split_k > 1 ? launch_split_reduce<!B_KC>(stream, p, e) : RST_OK;
+    }
+  }
   if (burst)
     hipLaunchKernelGGL((gemm_f64_mfma<BM, BN, WGM, WGN, A_KC, B_KC, VEC, (BM == 32 ? kBurst : 0)>),
                        dim3((unsigned)blocks), dim3(WGM * WGN * 64), 0, stream, p);
@@ -1435,16 +1639,17 @@ Route choose_route(const GemmParams& p, int* dma_slices, bool is_a_kc = false, b
 }
 
 template <bool A_KC, bool B_KC, bool VEC>
-int launch_layout(hipStream_t stream, const GemmParams& p) {
+int launch_layout(hipStream_t stream, const GemmParams& p, const ActEpilogue* e) {
   int slices = 0;
+  if (e && !A_KC) return fail(RST_ERR_UNSUPPORTED, "no activation epilogue for this layout");
   switch (choose_route(p, &slices, A_KC, B_KC)) {
-    case Route::kDma: return launch_dma<A_KC, B_KC>(stream, p);
-    case Route::kDmaSliced: return launch_dma<A_KC, B_KC>(stream, p, slices);
+    case Route::kDma: return launch_dma<A_KC, B_KC>(stream, p, 0, e);
+    case Route::kDmaSliced: return launch_dma<A_KC, B_KC>(stream, p, slices, e);
     case Route::kDma64:
-      if constexpr (A_KC) return launch_dma64<B_KC>(stream, p, slices);
+      if constexpr (A_KC) return launch_dma64<B_KC>(stream, p, slices, e);
       else return fail(RST_ERR_UNSUPPORTED, "no 64x64 direct-to-LDS kernel for this layout");
-    case Route::kTile128: return launch_one<128, 128, 2, 4, A_KC, B_KC, VEC>(stream, p);
-    default: return launch_one<32, 32, 2, 2, A_KC, B_KC, VEC>(stream, p, kSmallTileSplitBelow);
+    case Route::kTile128: return launch_one<128, 128, 2, 4, A_KC, B_KC, VEC>(stream, p, 256, 2048, e);
+    default: return launch_one<32, 32, 2, 2, A_KC, B_KC, VEC>(stream, p, kSmallTileSplitBelow, 2048, e);
   }
 }
 
@@ -1507,12 +1712,12 @@ int launch_gemm(hipStream_t stream, const GemmDesc& d) {
   const GemmParams p = make_params(d);
   const bool vec = desc_vec_ok(d);
   if (d.a_kc && d.b_kc)
-    return vec ? launch_layout<true, true, true>(stream, p) : launch_layout<true, true, false>(stream, p);
+    return vec ? launch_layout<true, true, true>(stream, p, d.act) : launch_layout<true, true, false>(stream, p, d.act);
   if (!d.a_kc && !d.b_kc)
-    return vec ? launch_layout<false, false, true>(stream, p) : launch_layout<false, false, false>(stream, p);
+    return vec ? launch_layout<false, false, true>(stream, p, d.act) : launch_layout<false, false, false>(stream, p, d.act);
   if (d.a_kc && !d.b_kc)
-    return vec ? launch_layout<true, false, true>(stream, p) : launch_layout<true, false, false>(stream, p);
-  return vec ? launch_layout<false, true, true>(stream, p) : launch_layout<false, true, false>(stream, p);
+    return vec ? launch_layout<true, false, true>(stream, p, d.act) : launch_layout<true, false, false>(stream, p, d.act);
+  return vec ? launch_layout<false, true, true>(stream, p, d.act) : launch_layout<false, true, false>(stream, p, d.act);
 }
 
 int max_gemm_group() { return kMaxGroup; }
@@ -1716,8 +1921,12 @@ int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count) {
   blocks = reduce_blocks = 0;
   size_t ws_used = 0;
   bool mixed = false;  // anything but weight-gradient layouts
+  const ActEpilogue* act = count == 2 ? d[1].act : nullptr;
+  if (act && (d[0].a_kc || d[0].b_kc || !d[1].a_kc || d[1].b_kc))
+    return fail(RST_ERR_INVALID_ARGUMENT, "an activation epilogue belongs to the input gradient behind a weight gradient");
   for (int i = 0; i < count; ++i) {
-    if (!can_group_gemm(d[i])) return fail(RST_ERR_INVALID_ARGUMENT, "contraction %d cannot join a group", i);
+    if (!can_group_gemm(d[i]) || (d[i].act && d[i].act != act))
+      return fail(RST_ERR_INVALID_ARGUMENT, "contraction %d cannot join a group", i);
     GemmParams p = make_params(d[i]);
     plan_group_member(p);
     g.first_block[i] = (int)blocks;
@@ -1741,8 +1950,12 @@ int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count) {
   g.first_reduce_block[count] = (int)reduce_blocks;
   const bool burst = blocks <= compute_units();
   RST_OBSERVE_GEMM(mixed ? GemmKernel::kStagedMixedGroup : GemmKernel::kStagedGroup, 32, 32, 2, 2, false, false, true,
-                   burst ? kBurst : 0, blocks, 256, nullptr, nullptr, 0, &g);
-  if (mixed && burst)
+                   burst ? kBurst : 0, blocks, 256, nullptr, nullptr, 0, &g, act != nullptr);
+  if (act && burst)
+    hipLaunchKernelGGL(gemm_f64_mfma_grads_act<kBurst>, dim3((unsigned)blocks), dim3(256), 0, stream, g, *act);
+  else if (act)
+    hipLaunchKernelGGL(gemm_f64_mfma_grads_act<0>, dim3((unsigned)blocks), dim3(256), 0, stream, g, *act);
+  else if (mixed && burst)
     hipLaunchKernelGGL((gemm_f64_mfma_mixed_group<kBurst>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
   else if (mixed)
     hipLaunchKernelGGL((gemm_f64_mfma_mixed_group<0>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
@@ -1752,8 +1965,11 @@ int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count) {
     hipLaunchKernelGGL((gemm_f64_mfma_group<false, false, 0>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
   RST_HIP(hipGetLastError());
   if (reduce_blocks > 0) {
-    RST_OBSERVE_GEMM(GemmKernel::kSplitReduceGroup, 0, 0, 0, 0, false, false, false, 0, reduce_blocks, 256, nullptr, nullptr, 0, &g);
-    hipLaunchKernelGGL(split_reduce_group_kernel, dim3((unsigned)reduce_blocks), dim3(256), 0, stream, g);
+    RST_OBSERVE_GEMM(GemmKernel::kSplitReduceGroup, 0, 0, 0, 0, false, false, false, 0, reduce_blocks, 256, nullptr, nullptr, 0, &g, act != nullptr);
+    if (act)
+      hipLaunchKernelGGL(split_reduce_grads_act_kernel, dim3((unsigned)reduce_blocks), dim3(256), 0, stream, g, *act);
+    else
+      hipLaunchKernelGGL(split_reduce_group_kernel, dim3((unsigned)reduce_blocks), dim3(256), 0, stream, g);
     RST_HIP(hipGetLastError());
   }
   return RST_OK;
@@ -1761,7 +1977,7 @@ int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count) {
 
 bool can_pair_gemm(const GemmDesc& input_grad, const GemmDesc& weight_grad) {
   long long b1 = 0, b2 = 0;
-  const bool layouts = input_grad.a_kc && !input_grad.b_kc && !weight_grad.a_kc && !weight_grad.b_kc;
+  const bool layouts = input_grad.a_kc && !input_grad.b_kc && !weight_grad.a_kc && !weight_grad.b_kc && !input_grad.act;
   // worth it when the input gradient alone would leave one workgroup per CU
   return layouts && takes_plain_dma(input_grad, &b1) && takes_plain_dma(weight_grad, &b2) && b1 < 512 &&
          b1 % 8 == 0 && b2 >= b1 && b1 + b2 <= 0x7fffffffLL;

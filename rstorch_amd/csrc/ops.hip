@@ -97,6 +97,44 @@ int engine_cross_entropy(rst_engine* e, double* row_loss, const double* pred, co
   return RST_OK;
 }
 
+int engine_linear_backward(rst_engine* e, const double* grad, const double* x, const double* weight,
+                           double* grad_weight, double* grad_bias, double* grad_input,
+                           const double* relu_mask_source, const ActEpilogue* input_act, size_t batch,
+                           size_t in_features, size_t out_features) {
+  const double n = (double)batch;
+  GemmDesc dw{};  // grad_weight[out,in] = (grad^T . x) / n
+  dw.A = grad; dw.B = x; dw.C = grad_weight;
+  dw.M = (int)out_features; dw.N = (int)in_features; dw.K = (int)batch;
+  dw.lda = (long)out_features; dw.ldb = (long)in_features; dw.ldc = (long)in_features;
+  dw.a_kc = false; dw.b_kc = false;
+  dw.epilogue = EPI_DIVIDE; dw.divisor = n;
+  // grad_bias[1,out] = colsum(grad) / n rides along in the same launch
+  dw.colsum = (in_features > 0 && batch > 0) ? grad_bias : nullptr;
+  dw.colsum_div = n;
+  dw.workspace = e->d_gemm_ws; dw.workspace_count = e->gemm_ws_count;
+  GemmDesc dx{};  // grad_input[batch,in] = grad . weight
+  dx.A = grad; dx.B = weight; dx.C = grad_input;
+  dx.M = (int)batch; dx.N = (int)in_features; dx.K = (int)out_features;
+  dx.lda = (long)out_features; dx.ldb = (long)in_features; dx.ldc = (long)in_features;
+  dx.a_kc = true; dx.b_kc = false;
+  dx.epilogue = relu_mask_source ? EPI_MASK : EPI_NONE;
+  dx.mask = relu_mask_source; dx.ldmask = (long)in_features;
+  dx.act = input_act;
+  dx.workspace = e->d_gemm_ws; dx.workspace_count = e->gemm_ws_count;
+  // two small products that do not depend on each other: one grid
+  const GemmDesc both[2] = {dw, dx};
+  if (grad_input && can_group_gemm(dw) && can_group_gemm(dx) &&
+      gemm_group_workspace(both, 2) <= e->gemm_ws_count) {
+    RST_TRY(launch_gemm_group(e->stream, both, 2));
+  } else {
+    RST_TRY(launch_gemm(e->stream, dw));
+    if (grad_input) RST_TRY(launch_gemm(e->stream, dx));
+  }
+  if (grad_bias && !dw.colsum)
+    RST_TRY(launch_column_mean(e->stream, grad, grad_bias, batch, out_features, n));
+  return RST_OK;
+}
+
 }  // namespace rst
 
 extern "C" {
@@ -133,37 +171,8 @@ int rst_linear_backward(rst_engine* e, const double* grad, const double* x, cons
   RST_TRY(check_dim(batch, "batch"));
   RST_TRY(check_dim(in_features, "in_features"));
   RST_TRY(check_dim(out_features, "out_features"));
-  const double n = (double)batch;
-  GemmDesc dw{};  // grad_weight[out,in] = (grad^T . x) / n
-  dw.A = grad; dw.B = x; dw.C = grad_weight;
-  dw.M = (int)out_features; dw.N = (int)in_features; dw.K = (int)batch;
-  dw.lda = (long)out_features; dw.ldb = (long)in_features; dw.ldc = (long)in_features;
-  dw.a_kc = false; dw.b_kc = false;
-  dw.epilogue = EPI_DIVIDE; dw.divisor = n;
-  // grad_bias[1,out] = colsum(grad) / n rides along in the same launch
-  dw.colsum = (in_features > 0 && batch > 0) ? grad_bias : nullptr;
-  dw.colsum_div = n;
-  dw.workspace = e->d_gemm_ws; dw.workspace_count = e->gemm_ws_count;
-  GemmDesc dx{};  // grad_input[batch,in] = grad . weight
-  dx.A = grad; dx.B = weight; dx.C = grad_input;
-  dx.M = (int)batch; dx.N = (int)in_features; dx.K = (int)out_features;
-  dx.lda = (long)out_features; dx.ldb = (long)in_features; dx.ldc = (long)in_features;
-  dx.a_kc = true; dx.b_kc = false;
-  dx.epilogue = relu_mask_source ? EPI_MASK : EPI_NONE;
-  dx.mask = relu_mask_source; dx.ldmask = (long)in_features;
-  dx.workspace = e->d_gemm_ws; dx.workspace_count = e->gemm_ws_count;
-  // two small products that do not depend on each other: one grid
-  const GemmDesc both[2] = {dw, dx};
-  if (grad_input && can_group_gemm(dw) && can_group_gemm(dx) &&
-      gemm_group_workspace(both, 2) <= e->gemm_ws_count) {
-    RST_TRY(launch_gemm_group(e->stream, both, 2));
-  } else {
-    RST_TRY(launch_gemm(e->stream, dw));
-    if (grad_input) RST_TRY(launch_gemm(e->stream, dx));
-  }
-  if (grad_bias && !dw.colsum)
-    RST_TRY(launch_column_mean(e->stream, grad, grad_bias, batch, out_features, n));
-  return RST_OK;
+  return engine_linear_backward(e, grad, x, weight, grad_weight, grad_bias, grad_input, relu_mask_source, nullptr,
+                                batch, in_features, out_features);
 }
 
 int rst_relu_forward(rst_engine* e, const double* x, double* out, size_t count) {

@@ -54,6 +54,7 @@ const char* kernel_name(GemmKernel k) {
   }
 }
 
+bool g_act = false;     // the launch carries the residual block's epilogue (no interior path; reads indexed as C)
 std::string g_context;  // what is being checked, for the failure message
 
 [[noreturn]] void bad(const char* fmt, ...) {
@@ -181,7 +182,8 @@ void check_write_block(const GemmParams& p, int tm, int tn, int row0, int col0, 
   const size_t out_limit = sliced ? (size_t)p.M * (size_t)p.N : c_limit;
   if (sliced && ws_slice_offset(p, split) + (size_t)p.M * p.N > (size_t)p.split_k * p.M * p.N)
     bad("slice %d ends beyond the partial-product area", split);
-  const bool uses_interior_path = interior && (sliced || p.epilogue != 3 /*EPI_DIVIDE*/ || p.divisor_reciprocal != 0.0);
+  const bool act = g_act && !sliced;
+  const bool uses_interior_path = interior && !act && (sliced || p.epilogue != 3 /*EPI_DIVIDE*/ || p.divisor_reciprocal != 0.0);
   for (int lane = 0; lane < 64; ++lane) {
     const int lr = lane & 15, lk = lane >> 4;
     if (uses_interior_path) {
@@ -214,6 +216,7 @@ void check_write_block(const GemmParams& p, int tm, int tn, int row0, int col0, 
             const int rc = row < p.M ? row : p.M - 1, cc = col < p.N ? col : p.N - 1;
             if (rc < 0 || cc < 0) bad("clamped epilogue index is negative");
             if (!sliced && p.epilogue == 4) in_range("mask read", (size_t)rc * p.ldmask + cc, 1, mask_limit);
+            if (act) in_range("source or residual read", (size_t)rc * p.ldc + cc, 1, c_limit);
             if (!sliced && p.sgd_parm) in_range("parameter read", (size_t)rc * p.ldc + cc, 1, c_limit);
             if (!sliced && (p.epilogue == 1 || p.epilogue == 2)) in_range("bias read", (size_t)cc, 1, (size_t)p.N);
             if (row < p.M && col < p.N) {
@@ -583,7 +586,7 @@ void check_group_blocks(const GemmGroup& g, const int* first, long long blocks) 
 std::string key_of(const GemmLaunch& l) {
   std::string k((const char*)&l.kernel, sizeof(l.kernel));
   auto add = [&](const void* p, size_t n) { k.append((const char*)p, n); };
-  add(&l.bm, sizeof(int)); add(&l.wgm, sizeof(int)); add(&l.a_kc, 1); add(&l.b_kc, 1); add(&l.vec, 1);
+  add(&l.bm, sizeof(int)); add(&l.wgm, sizeof(int)); add(&l.a_kc, 1); add(&l.b_kc, 1); add(&l.vec, 1); add(&l.act, 1);
   add(&l.blocks, sizeof(l.blocks)); add(&l.first_blocks, sizeof(int));
   auto add_params = [&](const GemmParams& p) {
     // the pointers matter only through their alignment
@@ -619,6 +622,7 @@ void observe_gemm_launch(const GemmLaunch& l) {
     ++g_skipped_repeats;
     return;
   }
+  g_act = l.act;
   switch (l.kernel) {
     case GemmKernel::kStaged:
       check_staged_problem(*l.p, l.bm, l.bn, l.wgm, l.wgn, l.a_kc, l.b_kc, l.vec, l.blocks);

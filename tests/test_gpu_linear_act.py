@@ -27,11 +27,11 @@ def data(batch, k, n):
             rng.standard_normal((batch, n)))
 
 
-def forward(engine, x, w, b, residual, kind, pre=True, shift=0):
+def forward(engine, x, w, b, residual, kind, pre=True, shift=0, in_place=False):
     batch, k = x.shape
     n = w.shape[0]
     dev = [guarded(engine, a, shift) for a in (x, w, b, residual)]
-    out = blank(engine, (batch, n), shift)
+    out = dev[3] if in_place else blank(engine, (batch, n), shift)
     z = blank(engine, (batch, n), shift) if pre else None
     check(engine.lib.rst_linear_act_forward(engine.handle, *[address(a) for a in dev], address(z), out.ptr, batch, k, n,
                                             ACTIVATIONS[kind]))
@@ -144,6 +144,30 @@ def test_activation_limits(engine, kind, limits):
     slope = out.get()[0]
     assert slope[0] == 0.0 and slope[1] == 1.0 and slope[3] == 0.0 and slope[4] == 1.0 and slope[5] == 0.0 and slope[6] == 1.0
     assert slope[2] == 0.0 if kind == "relu" else np.isnan(slope[2])
+
+
+def test_residual_in_place(engine):
+    for batch, k, n in ((1, 300, 77), (40, 130, 70), (300, 2048, 600)):
+        _, x, w, b, res = data(batch, k, n)
+        want = forward(engine, x, w, b, res, "gelu", pre=False)
+        assert np.array_equal(forward(engine, x, w, b, res, "gelu", pre=False, in_place=True), want)
+
+
+def test_input_gradient_in_place(engine):
+    """grad_input written over input_pre or over residual_grad, grad_pre over grad or pre."""
+    for batch, k, n in ((1, 300, 77), (40, 130, 70), (300, 2048, 600), (2050, 2046, 130)):
+        rng, x, w, _, g = data(batch, k, n)
+        pre, ip, res = rng.standard_normal((batch, n)), rng.standard_normal((batch, k)), rng.standard_normal((batch, k))
+        want = backward(engine, g, pre, "silu", x, w, ip, "gelu", res)
+        for over_input, over_grad in ((0, 0), (1, 1)):
+            dg, dpre, dx, dw, dip, dres = (guarded(engine, a) for a in (g, pre, x, w, ip, res))
+            gw, gb = blank(engine, (n, k)), blank(engine, (1, n))
+            gp, gi = (dg, dpre)[over_grad], (dip, dres)[over_input]
+            check(engine.lib.rst_linear_act_backward(
+                engine.handle, dg.ptr, dpre.ptr, ACTIVATIONS["silu"], gp.ptr, dx.ptr, dw.ptr, gw.ptr, gb.ptr, gi.ptr, dip.ptr,
+                ACTIVATIONS["gelu"], dres.ptr, batch, k, n))
+            for a, b in zip((gp, gw, gb, gi), want):
+                assert np.array_equal(a.get(), b)
 
 
 def test_special_values_stay_in_their_row(engine):
