@@ -17,7 +17,7 @@ LIB_PATH = os.path.join(LIB_DIR, "librstorch_hip.so")
 
 SOURCES = ["engine.hip", "gemm_f64.hip", "streaming.hip", "softmax_ce.hip", "rng_fill.hip",
            "ops.hip", "model.hip", "staging.hip", "static_scratch.hip", "elementwise.hip", "layer_norm.hip",
-           "block_ops.hip"]
+           "linear_rows.hip", "block_ops.hip"]
 
 HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",

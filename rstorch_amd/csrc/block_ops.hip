@@ -101,6 +101,8 @@ int rst_linear_act_forward(rst_engine* e, const double* x, const double* weight,
   RST_TRY(check_dim("linear_act_forward", in_features, "in_features"));
   RST_TRY(check_dim("linear_act_forward", out_features, "out_features"));
   const ActEpilogue act{activation, nullptr, residual, pre_out};
+  if (linear_rows_supported(batch, out_features, in_features))
+    return launch_linear_rows(e->stream, x, weight, bias, out, act, batch, out_features, in_features);
   GemmDesc d{};
   d.A = x; d.B = weight; d.C = out;
   d.M = (int)batch; d.N = (int)out_features; d.K = (int)in_features;
@@ -137,9 +139,8 @@ int rst_linear_act_backward(rst_engine* e, const double* grad, const double* pre
     grad = grad_pre;
   }
   const ActEpilogue act{input_activation, input_pre, residual_grad, nullptr};
-  const bool plain = input_activation == RST_ACT_NONE && !residual_grad;
-  return engine_linear_backward(e, grad, x, weight, grad_weight, grad_bias, grad_input, nullptr, plain ? nullptr : &act,
-                                batch, in_features, out_features);
+  return engine_linear_backward(e, grad, x, weight, grad_weight, grad_bias, grad_input, nullptr, &act, batch,
+                                in_features, out_features);
 }
 
 }  // extern "C"

@@ -89,6 +89,14 @@ int launch_gemm(hipStream_t stream, const GemmDesc& d);
 // under-fill the chip (fewer than 512 tiles).
 bool can_pair_gemm(const GemmDesc& input_grad, const GemmDesc& weight_grad);
 int launch_gemm_pair(hipStream_t stream, const GemmDesc& input_grad, const GemmDesc& weight_grad);
+// A layer's weight gradient and its input gradient with an ActEpilogue in one grid, as launch_gemm_pair.
+bool can_pair_grads_act(const GemmDesc& weight_grad, const GemmDesc& input_grad);
+int launch_gemm_grads_act(hipStream_t stream, const GemmDesc& weight_grad, const GemmDesc& input_grad);
+// out[rows, features] = act(x[rows, length] . w[features, length]^T + bias) + residual for a few rows, where
+// that beats the matrix tiles (linear_rows_supported)
+bool linear_rows_supported(size_t rows, size_t features, size_t length);
+int launch_linear_rows(hipStream_t s, const double* x, const double* w, const double* bias, double* out,
+                       const ActEpilogue& e, size_t rows, size_t features, size_t length);
 // Several small weight gradients (both operands output-contiguous, each a launch of 32x32 tiles
 // on its own, with or without K slices) in one grid, plus one shared reduction grid for the
 // sliced ones; same results as launch_gemm on each, except that from a batch of about 4096 a

@@ -23,6 +23,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <type_traits>
+#include <utility>
 
 #include "activation.h"
 #include "common.h"
@@ -1208,6 +1209,21 @@ __global__ __launch_bounds__(512, 4) void gemm_f64_mfma_dma_pair(const GemmParam
     dma_tile<A_KC2, B_KC2, 2, 4, 2, 1>(second, slot.block, lds_a, lds_b);
 }
 
+// A layer's weight gradient and its input gradient with the epilogue in one grid of 128x128 tiles.  The one with
+// fewer tiles comes first (DX_FIRST: the input gradient); the other's tiles fill the second slot of every CU.
+template <bool DX_FIRST>
+__global__ __launch_bounds__(512, 4) void gemm_f64_mfma_dma_grads_act(const GemmParams first, const GemmParams second,
+                                                                     int first_blocks, const ActEpilogue e) {
+  __shared__ __attribute__((aligned(1024))) double lds_a[2 * kDmaStage];
+  __shared__ __attribute__((aligned(1024))) double lds_b[2 * kDmaStage];
+  const PairSlot slot = pair_slot_of_block((int)blockIdx.x, first_blocks);
+  const ActFinish<true> finish{e};
+  if ((slot.problem == 0) == DX_FIRST)
+    dma_tile<true, false, 2, 4, 2, 1, false>(DX_FIRST ? first : second, slot.block, lds_a, lds_b, finish);
+  else
+    dma_tile<false, false, 2, 4, 2, 1>(DX_FIRST ? second : first, slot.block, lds_a, lds_b);
+}
+
 // Sum of `count` values `stride` doubles apart, added in order; up to 32 loads are in flight at a
 // time (the slices were written by other XCDs, so every load is a trip to memory).
 __device__ __forceinline__ double ordered_slice_sum(const double* __restrict__ first, size_t stride, int count) {
@@ -1638,10 +1654,60 @@ Route choose_route(const GemmParams& p, int* dma_slices, bool is_a_kc = false, b
   return Route::kTile32;
 }
 
+// Tiles and K slices of a product with the residual block's epilogue, where choose_route sends it to the
+// direct-to-LDS kernels at all: the cheapest of 128x128 tiles on up to 8 slices and 64x64 tiles on up to 16, by
+// a model in microseconds fitted to this part on fourteen shapes (32 to 144 tiles of 128x128, K = 1500 to 4096;
+// every one of them timed with 2 to 8 slices of either tile):
+//   512 workgroups are in flight, two per CU; a K step of 128x128 takes 1.84 while a CU has one workgroup and
+//   3.65 while it has two, a step of 64x64 0.535 and 1.0; later workgroups start as earlier ones leave; 6 for
+//   the launch; a slice more writes and reads M N doubles at 5.2 TB/s.
+// It is within 6 % of the measured time of nearly every one of them, and what it picks is within 3 % of the best: 1023 x 1023
+// at K = 4095 140 us on four slices (159 on the seven that choose_route takes), 768 x 1536 at K = 2048 91 (132),
+// 1500 x 1500 at K = 1500 135 (153), 700 x 700 at K = 3000 59 (66); 1024 x 1024 at K = 4096 137 (144).
+// choose_route itself keeps its slices: the order of the plain products' summation does not change.
+// Constants, not the device's own counts, for the same reason.
+struct ActPlan {
+  int tile, slices;  // tile 0: as choose_route says
+};
+ActPlan plan_act(const GemmParams& p, bool a_kc, bool b_kc) {
+  int slices = 0;
+  const Route route = choose_route(p, &slices, a_kc, b_kc);
+  ActPlan best{0, 1};
+  // (the model knows nothing of outputs that are mostly padding and bound by the weights' bytes)
+  if (route == Route::kTile32 || route == Route::kTile128 || p.M < 128 || p.N < 128) return best;
+  const int nk = dma_whole_steps(p.K, p.k_reserve);
+  double best_cost = 0.0;
+  auto consider = [&](int tile, int max_slices, double one, double two) {
+    const long long tiles = (long long)((p.M + tile - 1) / tile) * ((p.N + tile - 1) / tile);
+    for (int s = 1; s <= max_slices; ++s) {
+      if (s > 1 && (nk / s < 8 || p.ws == nullptr || p.ws_capacity < (size_t)s * ((size_t)p.M * p.N + (size_t)p.M))) break;
+      const int steps = (nk + s - 1) / s;
+      const long long groups = tiles * s, rem = groups % 512;
+      double c = 6.0 + (double)(groups / 512) * two * steps + (rem > 256 ? two * steps : rem > 0 ? one * steps : 0.0);
+      if (s > 1) c += 16.0 * s * (double)p.M * (double)p.N / 5.2e6;
+      if (best.tile == 0 || c < 0.98 * best_cost) {
+        best = ActPlan{tile, s};
+        best_cost = c;
+      }
+    }
+  };
+  consider(128, 8, 1.84, 3.65);
+  // (from 512 tiles on the larger ones have the chip full, and the smaller would read every operand twice as often)
+  if (a_kc && (long long)((p.M + 127) / 128) * ((p.N + 127) / 128) < 512) consider(64, 16, 0.535, 1.0);
+  return best;
+}
+
 template <bool A_KC, bool B_KC, bool VEC>
 int launch_layout(hipStream_t stream, const GemmParams& p, const ActEpilogue* e) {
   int slices = 0;
   if (e && !A_KC) return fail(RST_ERR_UNSUPPORTED, "no activation epilogue for this layout");
+  if (e) {
+    const ActPlan plan = plan_act(p, A_KC, B_KC);
+    if constexpr (A_KC) {
+      if (plan.tile == 64) return launch_dma64<B_KC>(stream, p, plan.slices, e);
+    }
+    if (plan.tile == 128) return launch_dma<A_KC, B_KC>(stream, p, plan.slices, e);
+  }
   switch (choose_route(p, &slices, A_KC, B_KC)) {
     case Route::kDma: return launch_dma<A_KC, B_KC>(stream, p, 0, e);
     case Route::kDmaSliced: return launch_dma<A_KC, B_KC>(stream, p, slices, e);
@@ -1993,6 +2059,36 @@ int launch_gemm_pair(hipStream_t stream, const GemmDesc& input_grad, const GemmD
   RST_OBSERVE_GEMM(GemmKernel::kDma128Pair, 128, 128, 2, 4, true, false, true, 0, b1 + b2, 512, &p1, &p2, (int)b1, nullptr);
   hipLaunchKernelGGL((gemm_f64_mfma_dma_pair<true, false, false, false>), dim3((unsigned)(b1 + b2)), dim3(512),
                      0, stream, p1, p2, (int)b1);
+  RST_HIP(hipGetLastError());
+  return RST_OK;
+}
+
+bool can_pair_grads_act(const GemmDesc& weight_grad, const GemmDesc& input_grad) {
+  long long b1 = 0, b2 = 0;
+  if (!input_grad.act || !input_grad.a_kc || input_grad.b_kc || weight_grad.a_kc || weight_grad.b_kc) return false;
+  if (!takes_plain_dma(weight_grad, &b1) || !takes_plain_dma(input_grad, &b2)) return false;
+  if (b1 > b2) std::swap(b1, b2);
+  return b1 < 512 && b1 % 8 == 0 && b1 + b2 <= 0x7fffffffLL;
+}
+
+int launch_gemm_grads_act(hipStream_t stream, const GemmDesc& weight_grad, const GemmDesc& input_grad) {
+  if (!can_pair_grads_act(weight_grad, input_grad))
+    return fail(RST_ERR_INVALID_ARGUMENT, "these two contractions cannot share a grid");
+  GemmParams dw = make_params(weight_grad), dx = make_params(input_grad);
+  for (GemmParams* p : {&dw, &dx}) {
+    p->tiles_m = (p->M + 127) / 128;
+    p->tiles_n = (p->N + 127) / 128;
+    p->steps_per_split = dma_whole_steps(p->K, p->k_reserve);
+  }
+  const long long bw = (long long)dw.tiles_m * dw.tiles_n, bx = (long long)dx.tiles_m * dx.tiles_n;
+  const dim3 grid((unsigned)(bw + bx));
+  if (bx <= bw) {
+    RST_OBSERVE_GEMM(GemmKernel::kDma128Pair, 128, 128, 2, 4, true, false, true, 0, bw + bx, 512, &dx, &dw, (int)bx, nullptr, true);
+    hipLaunchKernelGGL(gemm_f64_mfma_dma_grads_act<true>, grid, dim3(512), 0, stream, dx, dw, (int)bx, *input_grad.act);
+  } else {
+    RST_OBSERVE_GEMM(GemmKernel::kDma128Pair, 128, 128, 2, 4, false, false, true, 0, bw + bx, 512, &dw, &dx, (int)bw, nullptr, true);
+    hipLaunchKernelGGL(gemm_f64_mfma_dma_grads_act<false>, grid, dim3(512), 0, stream, dw, dx, (int)bw, *input_grad.act);
+  }
   RST_HIP(hipGetLastError());
   return RST_OK;
 }

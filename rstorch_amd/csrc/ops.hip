@@ -126,6 +126,8 @@ int engine_linear_backward(rst_engine* e, const double* grad, const double* x, c
   if (grad_input && can_group_gemm(dw) && can_group_gemm(dx) &&
       gemm_group_workspace(both, 2) <= e->gemm_ws_count) {
     RST_TRY(launch_gemm_group(e->stream, both, 2));
+  } else if (grad_input && can_pair_grads_act(dw, dx)) {
+    RST_TRY(launch_gemm_grads_act(e->stream, dw, dx));
   } else {
     RST_TRY(launch_gemm(e->stream, dw));
     if (grad_input) RST_TRY(launch_gemm(e->stream, dx));

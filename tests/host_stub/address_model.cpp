@@ -652,8 +652,11 @@ void observe_gemm_launch(const GemmLaunch& l) {
         if ((s.block & 7) != (b & 7)) bad("workgroup %lld runs block %d: another XCD than the tile walk assumes", b, s.block);
       }
       if (l.p->split_k != 1 || l.p2->split_k != 1) bad("a paired product is split");
-      check_dma128_problem(*l.p, true, false, b1);
-      check_dma128_problem(*l.p2, false, false, b2);
+      // the input gradient (A contraction-contiguous) carries the epilogue; it is the first unless l.a_kc says otherwise
+      g_act = l.act && l.a_kc;
+      check_dma128_problem(*l.p, l.a_kc, false, b1);
+      g_act = l.act && !l.a_kc;
+      check_dma128_problem(*l.p2, !l.a_kc, false, b2);
       break;
     }
     case GemmKernel::kDma128Group: {

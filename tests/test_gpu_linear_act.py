@@ -1,6 +1,9 @@
 """rst_linear_act_forward / _backward and rst_activation_* through the C ABI, element by element."""
+import math
+
 import numpy as np
 import pytest
+from scipy.special import erfc
 
 from block_reference import (ACT_CURVE, ACTIVATIONS, U, act, act_bound, address, blank, guarded, linear_backward,
                              linear_forward, within)
@@ -128,6 +131,30 @@ def test_activation_passes(engine, kind, count):
             check(engine.lib.rst_activation_backward(engine.handle, dg.ptr, dz.ptr, address(dr), out.ptr, count,
                                                      ACTIVATIONS[kind]))
             within(out.get(), g * slope + add, np.abs(g) * act_bound(z) + 2 * U * (np.abs(g * slope) + np.abs(add)), "gradient")
+
+
+@pytest.mark.parametrize("kind", ["gelu", "gelu_tanh", "silu"])
+def test_activations_over_their_range(engine, kind):
+    """Values and derivatives from -45 to 45 and around 0, against longdouble arithmetic: the exponential is within 3 U of
+    its value times max(1, its argument), which a factor exp(-argument) keeps below 3 U absolutely; the reciprocals and
+    polynomials (at most 1/2 in value, slope 1 in an argument of 3 roundings) add 4 U, the cubic argument of the tanh form 4 U
+    more: 16 U max(1, |z|)."""
+    z = np.concatenate([np.linspace(-45, 45, 20011), np.linspace(-1e-3, 1e-3, 999), -np.logspace(-300, 0, 500)]).reshape(1, -1)
+    zl = z.astype(np.longdouble)
+    if kind == "gelu":
+        p = np.where(z > 0, 1.0 - 0.5 * erfc(z / math.sqrt(2.0)).astype(np.longdouble), 0.5 * erfc(-z / math.sqrt(2.0)))
+        want, slope = zl * p, p + zl * np.exp(-zl * zl / 2) / np.sqrt(2 * np.longdouble(math.pi))
+    else:
+        c = 2 * np.sqrt(2 / np.longdouble(math.pi))
+        a = np.longdouble(0.044715)
+        t, dt = (zl, 1) if kind == "silu" else (c * (zl + a * zl ** 3), c * (1 + 3 * a * zl * zl))
+        s = 1 / (1 + np.exp(-t))
+        want, slope = zl * s, s + zl * s * (1 / (1 + np.exp(t))) * dt
+    dz, one, out = guarded(engine, z), guarded(engine, np.ones_like(z)), blank(engine, z.shape)
+    check(engine.lib.rst_activation_forward(engine.handle, dz.ptr, None, out.ptr, z.size, ACTIVATIONS[kind]))
+    within(out.get(), want, 16 * U * np.maximum(1.0, np.abs(z)), "value")
+    check(engine.lib.rst_activation_backward(engine.handle, one.ptr, dz.ptr, None, out.ptr, z.size, ACTIVATIONS[kind]))
+    within(out.get(), slope, 16 * U * np.maximum(1.0, np.abs(z)), "derivative")
 
 
 @pytest.mark.parametrize("kind,limits", [("relu", (0.0, np.inf, 0.0)), ("gelu", (0.0, np.inf, np.nan)),
