@@ -198,37 +198,81 @@ __global__ __launch_bounds__(BLOCK, WAVES) void norm_forward_kernel(const double
   }
 }
 
-// Rows of one value (no pair to load), and rows too wide for the registers: one workgroup walks the row
-// three times (mean, variance, result).
+// Rows too wide for the registers, and rows of one value (no pair to load): one workgroup walks the row twice.  The
+// first walk takes mean and squared deviations together: a thread's batch of sixteen values gets its own mean and
+// deviations in registers (no cancellation), which join the thread's running ones; the threads' means then give the
+// row's, and the deviations are moved onto it: sum_i (S_i + n_i (m_i - m)^2).  All of this is done on x minus the row's
+// first value, which is within sqrt(cols) standard deviations of the mean: a rounding of the means is then small
+// against the deviations also where the values have a large common part.  1024 x 32768: 171 us (184 in three
+// walks; 207 with the row kept half in registers and half in LDS, which leaves one workgroup per CU and nothing to overlap
+// its phases with).
 template <int BLOCK>
 __global__ __launch_bounds__(BLOCK) void norm_forward_wide_kernel(const double* x, const double* __restrict__ w,
                                                                   const double* __restrict__ b, double* out,
                                                                   double* mean, double* rstd, size_t rows, size_t cols,
                                                                   double eps) {
   __shared__ double scratch[2][BLOCK / 64];
+  constexpr size_t STEP = 2 * BLOCK;
+  constexpr int DEPTH = 8;
   const double n = (double)cols;
   for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const double* src = x + row * cols;
-    double sum = 0.0;
-    for (size_t c = 2 * (size_t)threadIdx.x; c < cols; c += 2 * BLOCK) {
-      const v2u v = load_pair(src, c, cols);
-      sum += v.x + v.y;
+    const double shift = src[0];
+    double count = 0.0, centre = 0.0, spread = 0.0;  // of what this thread has read
+    // joins `values` more values of the given mean and squared deviations
+    auto join = [&](double values, double m, double s) {
+      const double total = count + values, delta = m - centre;
+      const double share = values / total;
+      centre = fma(delta, share, centre);
+      spread += fma(delta * delta, count * share, s);
+      count = total;
+    };
+    size_t c = 2 * (size_t)threadIdx.x;
+    for (; c + (DEPTH - 1) * STEP + 1 < cols; c += DEPTH * STEP) {
+      v2u t[DEPTH];
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) t[d] = load2(src + c + d * STEP);
+      double sum = 0.0, sq = 0.0;
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        t[d] -= shift;
+        sum += t[d].x + t[d].y;
+      }
+      const double m = sum * (0.5 / DEPTH);
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        sq = fma(t[d].x - m, t[d].x - m, sq);
+        sq = fma(t[d].y - m, t[d].y - m, sq);
+      }
+      join(2.0 * DEPTH, m, sq);
     }
-    const double m = group_sum<BLOCK>(sum, scratch[0]) / n;
-    double sq = 0.0;
-    for (size_t c = 2 * (size_t)threadIdx.x; c < cols; c += 2 * BLOCK) {
-      const v2u v = load_pair(src, c, cols);
-      const double d0 = v.x - m, d1 = c + 1 < cols ? v.y - m : 0.0;
-      sq = fma(d0, d0, sq);
-      sq = fma(d1, d1, sq);
+    for (; c < cols; c += STEP) {
+      const v2u t = load_pair(src, c, cols) - shift;
+      if (c + 1 < cols) {
+        const double half = 0.5 * (t.x - t.y);
+        join(2.0, t.y + half, 2.0 * half * half);
+      } else {
+        join(1.0, t.x, 0.0);
+      }
     }
-    const double r = 1.0 / sqrt(group_sum<BLOCK>(sq, scratch[1]) / n + eps);
-    for (size_t c = 2 * (size_t)threadIdx.x; c < cols; c += 2 * BLOCK) {
-      v2u y = (load_pair(src, c, cols) - m) * r;
-      if (w) y *= load_pair(w, c, cols);
-      if (b) y += load_pair(b, c, cols);
-      store_pair(out + row * cols, c, cols, y);
+    const double moved = group_sum<BLOCK>(count * centre, scratch[0]) / n;
+    const double m = shift + moved, off = centre - moved;
+    const double r = 1.0 / sqrt(group_sum<BLOCK>(fma(count * off, off, spread), scratch[1]) / n + eps);
+    c = 2 * (size_t)threadIdx.x;
+    auto finish = [&](v2u v, size_t at) {
+      v2u y = (v - m) * r;
+      if (w) y *= load_pair(w, at, cols);
+      if (b) y += load_pair(b, at, cols);
+      store_pair(out + row * cols, at, cols, y);
+    };
+    for (; c + 3 * STEP + 1 < cols; c += 4 * STEP) {
+      v2u t[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) t[d] = load2(src + c + d * STEP);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) finish(t[d], c + d * STEP);
     }
+    for (; c < cols; c += STEP) finish(load_pair(src, c, cols), c);
     if (threadIdx.x == 0) {
       if (mean) mean[row] = m;
       if (rstd) rstd[row] = r;
@@ -490,8 +534,8 @@ template <int BLOCK>
 int forward_wide(hipStream_t s, const double* x, const double* w, const double* b, double* out, double* mean,
                  double* rstd, size_t rows, size_t cols, double eps) {
   const size_t most = ((size_t)1 << 31) / BLOCK;  // (a grid has fewer than 2^32 threads)
-  hipLaunchKernelGGL(norm_forward_wide_kernel<BLOCK>, dim3((unsigned)(rows < most ? rows : most)), dim3(BLOCK), 0, s,
-                     x, w, b, out, mean, rstd, rows, cols, eps);
+  hipLaunchKernelGGL((norm_forward_wide_kernel<BLOCK>), dim3((unsigned)(rows < most ? rows : most)),
+                     dim3(BLOCK), 0, s, x, w, b, out, mean, rstd, rows, cols, eps);
   RST_HIP(hipGetLastError());
   return RST_OK;
 }
