@@ -1477,13 +1477,42 @@ void plan_slices(GemmParams& p, long long blocks, long long split_below, long lo
   }
 }
 
+// Slices of 32x32 tiles with the residual block's epilogue, by a model in microseconds: a K step takes a workgroup
+// 0.27, workgroups beyond one per CU wait their turn, and slices need a second launch.  On batches and widths of 15 to
+// 2500 and inner dimensions of 64 to 1024, each timed whole and sliced: 32 x 128 -> 100 takes 6.0 us whole and 6.6
+// sliced, 32 x 1024 -> 100 10.9 and 7.2; both gradients of 32 -> 100 features 6.4 and 9.5 at a batch of 128, 26.6 and
+// 10.6 at 1024.  second_launch: what it costs.  others: workgroups of the same grid that are not this product's.
+void plan_act_slices(GemmParams& p, long long blocks, long long others, double second_launch) {
+  const int nk = (p.K + BK - 1) / BK;
+  p.split_k = 1;
+  p.steps_per_split = nk;
+  if (p.ws == nullptr) return;
+  const long long room = (long long)(p.ws_capacity / ((size_t)p.M * p.N + (size_t)p.M));
+  double best = 0.0;
+  long long slices = 1;
+  for (long long s = 1; s <= 64 && (s == 1 || (nk / s >= 4 && s <= room)); ++s) {
+    const double rounds = (double)((blocks * s + others + 255) / 256);
+    const double c = 0.27 * (double)((nk + s - 1) / s) * rounds + (s > 1 ? second_launch : 0.0);
+    if (s == 1 || c < best - 0.1) {
+      best = c;
+      slices = s;
+    }
+  }
+  if (slices > 1) {
+    p.steps_per_split = (int)((nk + slices - 1) / slices);
+    p.split_k = (nk + p.steps_per_split - 1) / p.steps_per_split;
+    p.ws_colsum = p.ws + (size_t)p.split_k * p.M * p.N;
+  }
+}
+
 template <int BM, int BN, int WGM, int WGN, bool A_KC, bool B_KC, bool VEC>
 int launch_one(hipStream_t stream, GemmParams p, long long split_below = 256, long long want_blocks = 2048,
                const ActEpilogue* e = nullptr) {
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
   long long blocks = (long long)p.tiles_m * p.tiles_n;
-  plan_slices(p, blocks, split_below, want_blocks);
+  if (e && BM == 32) plan_act_slices(p, blocks, 0, 2.6);
+  else plan_slices(p, blocks, split_below, want_blocks);
   blocks *= p.split_k;
   if (blocks > 0x7fffffffLL) return fail(RST_ERR_UNSUPPORTED, "contraction grid too large");
   const bool burst = BM == 32 && BN == 32 && blocks <= compute_units();
@@ -1789,11 +1818,18 @@ int launch_gemm(hipStream_t stream, const GemmDesc& d) {
 int max_gemm_group() { return kMaxGroup; }
 
 namespace {
-// the slices of a group member: what launch_gemm would choose for it alone
-void plan_group_member(GemmParams& p) {
+// the slices of member i of a group: what launch_gemm would choose for it alone; with the residual block's epilogue in
+// the group, by the model of plan_act_slices
+void plan_group_member(GemmParams& p, const GemmDesc* d, int count, int i) {
   p.tiles_m = (p.M + 31) / 32;
   p.tiles_n = (p.N + 31) / 32;
-  plan_slices(p, (long long)p.tiles_m * p.tiles_n, kSmallTileSplitBelow, 2048);
+  const long long tiles = (long long)p.tiles_m * p.tiles_n;
+  if (count == 2 && d[1].act) {
+    const GemmDesc& other = d[1 - i];
+    plan_act_slices(p, tiles, (long long)((other.M + 31) / 32) * ((other.N + 31) / 32), 3.9);
+  } else {
+    plan_slices(p, tiles, kSmallTileSplitBelow, 2048);
+  }
 }
 }  // namespace
 
@@ -1960,7 +1996,7 @@ size_t gemm_group_workspace(const GemmDesc* d, int count) {
   size_t need = 0;
   for (int i = 0; i < count; ++i) {
     GemmParams p = make_params(d[i]);
-    plan_group_member(p);
+    plan_group_member(p, d, count, i);
     if (p.split_k > 1) need += (size_t)p.split_k * ((size_t)p.M * p.N + (size_t)p.M);
   }
   return need;
@@ -1994,7 +2030,7 @@ int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count) {
     if (!can_group_gemm(d[i]) || (d[i].act && d[i].act != act))
       return fail(RST_ERR_INVALID_ARGUMENT, "contraction %d cannot join a group", i);
     GemmParams p = make_params(d[i]);
-    plan_group_member(p);
+    plan_group_member(p, d, count, i);
     g.first_block[i] = (int)blocks;
     g.first_reduce_block[i] = (int)reduce_blocks;
     g.layout[i] = (unsigned char)((d[i].a_kc ? 1 : 0) | (d[i].b_kc ? 2 : 0));

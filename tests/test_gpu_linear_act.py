@@ -197,6 +197,23 @@ def test_input_gradient_in_place(engine):
                 assert np.array_equal(a.get(), b)
 
 
+def test_one_gradient_in_three_places(engine):
+    """The residual block in place: the gradient that arrives is also the skipped one and where the result goes."""
+    for batch, n in ((1, 40), (20, 40), (32, 100), (130, 33), (300, 600)):
+        rng, x, w, _, g = data(batch, n, n)
+        pre = rng.standard_normal((batch, n))
+        want = backward(engine, g, pre, "gelu", x, w, None, "none", g)
+        for grad_pre_over_pre in (False, True):
+            dg, dpre, dx, dw = (guarded(engine, a) for a in (g, pre, x, w))
+            gw, gb, gp = blank(engine, (n, n)), blank(engine, (1, n)), blank(engine, (batch, n))
+            gp = dpre if grad_pre_over_pre else gp
+            check(engine.lib.rst_linear_act_backward(
+                engine.handle, dg.ptr, dpre.ptr, ACTIVATIONS["gelu"], gp.ptr, dx.ptr, dw.ptr, gw.ptr, gb.ptr, dg.ptr, None,
+                ACTIVATIONS["none"], dg.ptr, batch, n, n))
+            for a, b in zip((gp, gw, gb, dg), want):
+                assert np.array_equal(a.get(), b)
+
+
 def test_special_values_stay_in_their_row(engine):
     """A NaN or an infinity in one row of x reaches that row of the result and no other."""
     for batch, k, n in ((1, 64, 64), (6, 200, 90), (64, 500, 64), (600, 600, 200)):
