@@ -106,6 +106,7 @@ int launch_linear_rows(hipStream_t s, const double* x, const double* w, const do
 // layer's input gradient, which carries it.
 bool can_group_gemm(const GemmDesc& d);
 size_t gemm_group_workspace(const GemmDesc* d, int count);
+bool can_group_grads_act(const GemmDesc* d);  // d[0] a weight gradient, d[1] the input gradient with an ActEpilogue
 int max_gemm_group();
 int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count);
 

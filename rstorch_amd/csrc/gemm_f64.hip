@@ -1477,32 +1477,49 @@ void plan_slices(GemmParams& p, long long blocks, long long split_below, long lo
   }
 }
 
-// Slices of 32x32 tiles with the residual block's epilogue, by a model in microseconds: a K step takes a workgroup
-// 0.27, workgroups beyond one per CU wait their turn, and slices need a second launch.  On batches and widths of 15 to
-// 2500 and inner dimensions of 64 to 1024, each timed whole and sliced: 32 x 128 -> 100 takes 6.0 us whole and 6.6
-// sliced, 32 x 1024 -> 100 10.9 and 7.2; both gradients of 32 -> 100 features 6.4 and 9.5 at a batch of 128, 26.6 and
-// 10.6 at 1024.  second_launch: what it costs.  others: workgroups of the same grid that are not this product's.
-void plan_act_slices(GemmParams& p, long long blocks, long long others, double second_launch) {
-  const int nk = (p.K + BK - 1) / BK;
-  p.split_k = 1;
-  p.steps_per_split = nk;
-  if (p.ws == nullptr) return;
-  const long long room = (long long)(p.ws_capacity / ((size_t)p.M * p.N + (size_t)p.M));
+// K slices of 32x32 tiles where the residual block's epilogue is in the grid (count 1: that product; 2: the weight and
+// the input gradient), by a model in microseconds: 3.7 for the launch, 0.14 per K step and CU and 0.59 per workgroup and CU,
+// 0.35 for each K step of the longest workgroup, 3.6 for the slices' second launch (2.6 behind one product).  All products
+// get slices of the same length, the cheapest.  Fitted to both gradients of eighteen layers (28 to 3111 rows, 3 to 3457 features), each timed on up to
+// 64 slices of either product: the picks are within 3 % of the best in the mean, 15 % at worst (1195 rows, 925 -> 8);
+// 3111 rows of 121 -> 442 take 30 us on 15 and 2 slices, 108 whole and 44 on as many as the plain products take.
+// Returns the modelled time.
+double plan_act_slices(GemmParams* const* p, int count) {
+  int nk[2] = {0, 0}, longest = 0;
+  long long tiles[2] = {0, 0};
+  size_t room = p[0]->ws != nullptr ? p[0]->ws_capacity : 0;
+  for (int i = 0; i < count; ++i) {
+    nk[i] = (p[i]->K + BK - 1) / BK;
+    tiles[i] = (long long)((p[i]->M + 31) / 32) * ((p[i]->N + 31) / 32);
+    if (nk[i] > longest) longest = nk[i];
+  }
+  const double join = count > 1 ? 3.6 : 2.6;
+  int steps = longest;
   double best = 0.0;
-  long long slices = 1;
-  for (long long s = 1; s <= 64 && (s == 1 || (nk / s >= 4 && s <= room)); ++s) {
-    const double rounds = (double)((blocks * s + others + 255) / 256);
-    const double c = 0.27 * (double)((nk + s - 1) / s) * rounds + (s > 1 ? second_launch : 0.0);
-    if (s == 1 || c < best - 0.1) {
+  for (int j = 1; j <= 64; ++j) {
+    const int n = (longest + j - 1) / j;
+    if (j > 1 && n < 3) break;
+    double work = 0.0, groups = 0.0;
+    size_t need = 0;
+    for (int i = 0; i < count; ++i) {
+      const int s = (nk[i] + n - 1) / n;
+      work += (double)tiles[i] * nk[i];
+      groups += (double)tiles[i] * s;
+      if (s > 1) need += (size_t)s * ((size_t)p[i]->M * p[i]->N + (size_t)p[i]->M);
+    }
+    if (j > 1 && need > room) break;
+    const double c = 3.7 + (0.14 * work + 0.59 * groups) / 256.0 + 0.35 * n + (j > 1 ? join : 0.0);
+    if (j == 1 || c < best) {
       best = c;
-      slices = s;
+      steps = n;
     }
   }
-  if (slices > 1) {
-    p.steps_per_split = (int)((nk + slices - 1) / slices);
-    p.split_k = (nk + p.steps_per_split - 1) / p.steps_per_split;
-    p.ws_colsum = p.ws + (size_t)p.split_k * p.M * p.N;
+  for (int i = 0; i < count; ++i) {
+    p[i]->steps_per_split = nk[i] < steps ? nk[i] : steps;
+    p[i]->split_k = nk[i] > steps ? (nk[i] + steps - 1) / steps : 1;
+    if (p[i]->split_k > 1) p[i]->ws_colsum = p[i]->ws + (size_t)p[i]->split_k * p[i]->M * p[i]->N;
   }
+  return best;
 }
 
 template <int BM, int BN, int WGM, int WGN, bool A_KC, bool B_KC, bool VEC>
@@ -1511,7 +1528,8 @@ int launch_one(hipStream_t stream, GemmParams p, long long split_below = 256, lo
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
   long long blocks = (long long)p.tiles_m * p.tiles_n;
-  if (e && BM == 32) plan_act_slices(p, blocks, 0, 2.6);
+  GemmParams* const self = &p;
+  if (e && BM == 32) plan_act_slices(&self, 1);
   else plan_slices(p, blocks, split_below, want_blocks);
   blocks *= p.split_k;
   if (blocks > 0x7fffffffLL) return fail(RST_ERR_UNSUPPORTED, "contraction grid too large");
@@ -1698,6 +1716,14 @@ Route choose_route(const GemmParams& p, int* dma_slices, bool is_a_kc = false, b
 struct ActPlan {
   int tile, slices;  // tile 0: as choose_route says
 };
+double dma_cost(const GemmParams& p, int tile, int slices) {
+  const double one = tile == 128 ? 1.84 : 0.535, two = tile == 128 ? 3.65 : 1.0;
+  const int nk = dma_whole_steps(p.K, p.k_reserve), steps = (nk + slices - 1) / slices;
+  const long long groups = (long long)((p.M + tile - 1) / tile) * ((p.N + tile - 1) / tile) * slices, rem = groups % 512;
+  double c = 6.0 + (double)(groups / 512) * two * steps + (rem > 256 ? two * steps : rem > 0 ? one * steps : 0.0);
+  if (slices > 1) c += 16.0 * slices * (double)p.M * (double)p.N / 5.2e6;
+  return c;
+}
 ActPlan plan_act(const GemmParams& p, bool a_kc, bool b_kc) {
   int slices = 0;
   const Route route = choose_route(p, &slices, a_kc, b_kc);
@@ -1706,23 +1732,19 @@ ActPlan plan_act(const GemmParams& p, bool a_kc, bool b_kc) {
   if (route == Route::kTile32 || route == Route::kTile128 || p.M < 128 || p.N < 128) return best;
   const int nk = dma_whole_steps(p.K, p.k_reserve);
   double best_cost = 0.0;
-  auto consider = [&](int tile, int max_slices, double one, double two) {
-    const long long tiles = (long long)((p.M + tile - 1) / tile) * ((p.N + tile - 1) / tile);
+  auto consider = [&](int tile, int max_slices) {
     for (int s = 1; s <= max_slices; ++s) {
       if (s > 1 && (nk / s < 8 || p.ws == nullptr || p.ws_capacity < (size_t)s * ((size_t)p.M * p.N + (size_t)p.M))) break;
-      const int steps = (nk + s - 1) / s;
-      const long long groups = tiles * s, rem = groups % 512;
-      double c = 6.0 + (double)(groups / 512) * two * steps + (rem > 256 ? two * steps : rem > 0 ? one * steps : 0.0);
-      if (s > 1) c += 16.0 * s * (double)p.M * (double)p.N / 5.2e6;
+      const double c = dma_cost(p, tile, s);
       if (best.tile == 0 || c < 0.98 * best_cost) {
         best = ActPlan{tile, s};
         best_cost = c;
       }
     }
   };
-  consider(128, 8, 1.84, 3.65);
+  consider(128, 8);
   // (from 512 tiles on the larger ones have the chip full, and the smaller would read every operand twice as often)
-  if (a_kc && (long long)((p.M + 127) / 128) * ((p.N + 127) / 128) < 512) consider(64, 16, 0.535, 1.0);
+  if (a_kc && (long long)((p.M + 127) / 128) * ((p.N + 127) / 128) < 512) consider(64, 16);
   return best;
 }
 
@@ -1818,18 +1840,20 @@ int launch_gemm(hipStream_t stream, const GemmDesc& d) {
 int max_gemm_group() { return kMaxGroup; }
 
 namespace {
-// the slices of member i of a group: what launch_gemm would choose for it alone; with the residual block's epilogue in
-// the group, by the model of plan_act_slices
-void plan_group_member(GemmParams& p, const GemmDesc* d, int count, int i) {
-  p.tiles_m = (p.M + 31) / 32;
-  p.tiles_n = (p.N + 31) / 32;
-  const long long tiles = (long long)p.tiles_m * p.tiles_n;
-  if (count == 2 && d[1].act) {
-    const GemmDesc& other = d[1 - i];
-    plan_act_slices(p, tiles, (long long)((other.M + 31) / 32) * ((other.N + 31) / 32), 3.9);
-  } else {
-    plan_slices(p, tiles, kSmallTileSplitBelow, 2048);
+// the parameters of a group of 32x32 tiles, its slices planned: what launch_gemm would choose for each member alone, or,
+// with the residual block's epilogue in the group, both by plan_act_slices
+void plan_group(const GemmDesc* d, int count, GemmParams* p) {
+  for (int i = 0; i < count; ++i) {
+    p[i] = make_params(d[i]);
+    p[i].tiles_m = (p[i].M + 31) / 32;
+    p[i].tiles_n = (p[i].N + 31) / 32;
   }
+  if (count == 2 && d[1].act) {
+    GemmParams* const both[2] = {&p[0], &p[1]};
+    plan_act_slices(both, 2);
+    return;
+  }
+  for (int i = 0; i < count; ++i) plan_slices(p[i], (long long)p[i].tiles_m * p[i].tiles_n, kSmallTileSplitBelow, 2048);
 }
 }  // namespace
 
@@ -1994,11 +2018,11 @@ size_t gemm_group_workspace(const GemmDesc* d, int count) {
     if (plan_dma_group(d, count, &g, &blocks, &reduce_blocks, &need)) return need;
   }
   size_t need = 0;
-  for (int i = 0; i < count; ++i) {
-    GemmParams p = make_params(d[i]);
-    plan_group_member(p, d, count, i);
-    if (p.split_k > 1) need += (size_t)p.split_k * ((size_t)p.M * p.N + (size_t)p.M);
-  }
+  if (count < 1 || count > kMaxGroup) return need;
+  GemmParams p[kMaxGroup];
+  plan_group(d, count, p);
+  for (int i = 0; i < count; ++i)
+    if (p[i].split_k > 1) need += (size_t)p[i].split_k * ((size_t)p[i].M * p[i].N + (size_t)p[i].M);
   return need;
 }
 
@@ -2026,11 +2050,12 @@ int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count) {
   const ActEpilogue* act = count == 2 ? d[1].act : nullptr;
   if (act && (d[0].a_kc || d[0].b_kc || !d[1].a_kc || d[1].b_kc))
     return fail(RST_ERR_INVALID_ARGUMENT, "an activation epilogue belongs to the input gradient behind a weight gradient");
+  GemmParams planned[kMaxGroup];
+  plan_group(d, count, planned);
   for (int i = 0; i < count; ++i) {
-    if (!can_group_gemm(d[i]) || (d[i].act && d[i].act != act))
+    if (!(act ? d[i].M > 0 && d[i].N > 0 : can_group_gemm(d[i])) || (d[i].act && d[i].act != act))
       return fail(RST_ERR_INVALID_ARGUMENT, "contraction %d cannot join a group", i);
-    GemmParams p = make_params(d[i]);
-    plan_group_member(p, d, count, i);
+    GemmParams& p = planned[i];
     g.first_block[i] = (int)blocks;
     g.first_reduce_block[i] = (int)reduce_blocks;
     g.layout[i] = (unsigned char)((d[i].a_kc ? 1 : 0) | (d[i].b_kc ? 2 : 0));
@@ -2075,6 +2100,29 @@ int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count) {
     RST_HIP(hipGetLastError());
   }
   return RST_OK;
+}
+
+// Both gradients of a layer in one grid of 32x32 tiles, or each on the tiles that suit it: whichever the two models
+// find shorter; the larger tiles from 3 GFLOP on.  On 46 layers of 0.25 to 10 GFLOP, each timed both ways, the pick is
+// within 1.3 % of the better in the mean, 10 % at worst: 1953 rows of 32 -> 3607 take 38 us together and 75 apart, 1462 of
+// 189 -> 529 29 and 38, 1024 of 1024 -> 1024 112 and 91.
+bool can_group_grads_act(const GemmDesc* d) {
+  if (!d[1].act || d[0].M <= 0 || d[0].N <= 0 || d[1].M <= 0 || d[1].N <= 0) return false;
+  if (4.0 * d[0].M * d[0].N * (double)d[0].K >= 3e9 || gemm_group_workspace(d, 2) > d[0].workspace_count) return false;
+  GemmParams p[2] = {make_params(d[0]), make_params(d[1])};
+  GemmParams* const both[2] = {&p[0], &p[1]};
+  const double together = plan_act_slices(both, 2);
+  double apart = 0.0;
+  for (int i = 0; i < 2; ++i) {
+    int slices = 0;
+    const Route route = choose_route(p[i], &slices, i == 1, false);
+    const ActPlan plan = i == 1 ? plan_act(p[i], true, false) : ActPlan{0, 1};
+    if (route == Route::kTile128) return false;
+    if (route == Route::kTile32) apart += plan_act_slices(&both[i], 1);
+    else if (plan.tile != 0) apart += dma_cost(p[i], plan.tile, plan.slices);
+    else apart += dma_cost(p[i], route == Route::kDma64 ? 64 : 128, slices > 1 ? slices : 1);
+  }
+  return together < apart;
 }
 
 bool can_pair_gemm(const GemmDesc& input_grad, const GemmDesc& weight_grad) {
