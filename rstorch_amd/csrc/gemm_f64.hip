@@ -1226,31 +1226,21 @@ __global__ __launch_bounds__(512, 4) void gemm_f64_mfma_dma_grads_act(const Gemm
 
 // Sum of `count` values `stride` doubles apart, added in order; up to 32 loads are in flight at a
 // time (the slices were written by other XCDs, so every load is a trip to memory).
+template <int IN_FLIGHT>
+__device__ __forceinline__ double add_slices(double v, const double* __restrict__ first, size_t stride, int count) {
+  double t[IN_FLIGHT];
+#pragma unroll
+  for (int j = 0; j < IN_FLIGHT; ++j) t[j] = first[j < count ? (size_t)j * stride : 0];
+#pragma unroll
+  for (int j = 0; j < IN_FLIGHT; ++j)
+    if (j < count) v += t[j];
+  return v;
+}
 __device__ __forceinline__ double ordered_slice_sum(const double* __restrict__ first, size_t stride, int count) {
   double v = 0.0;
-  int s = 0;
-  for (; s + 32 <= count; s += 32) {
-    double t[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) t[j] = first[(size_t)(s + j) * stride];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v += t[j];
-  }
-  for (; s + 8 <= count; s += 8) {
-    double t[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = first[(size_t)(s + j) * stride];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v += t[j];
-  }
-  if (s < count) {
-    double t[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = s + j < count ? first[(size_t)(s + j) * stride] : 0.0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (s + j < count) v += t[j];
-  }
+  for (; count > 16; count -= 32, first += 32 * stride) v = add_slices<32>(v, first, stride, count);
+  if (count > 8) v = add_slices<16>(v, first, stride, count);
+  else if (count > 0) v = add_slices<8>(v, first, stride, count);
   return v;
 }
 
@@ -1478,11 +1468,12 @@ void plan_slices(GemmParams& p, long long blocks, long long split_below, long lo
 }
 
 // K slices of 32x32 tiles where the residual block's epilogue is in the grid (count 1: that product; 2: the weight and
-// the input gradient), by a model in microseconds: 3.7 for the launch, 0.14 per K step and CU and 0.59 per workgroup and CU,
-// 0.35 for each K step of the longest workgroup, 3.6 for the slices' second launch (2.6 behind one product).  All products
-// get slices of the same length, the cheapest.  Fitted to both gradients of eighteen layers (28 to 3111 rows, 3 to 3457 features), each timed on up to
-// 64 slices of either product: the picks are within 3 % of the best in the mean, 15 % at worst (1195 rows, 925 -> 8);
-// 3111 rows of 121 -> 442 take 30 us on 15 and 2 slices, 108 whole and 44 on as many as the plain products take.
+// the input gradient), by a model in microseconds: 3.8 for the launch, 0.12 per K step and CU and 0.65 per workgroup and CU,
+// 0.35 for each K step of the longest workgroup; for slices 3.7 (2.6 behind one product) for the second launch, their bytes
+// and 2.1 beyond 32 of them, which that launch does not read in one go.  All products get slices of the same length, the
+// cheapest.  Fitted to both gradients of 37 layers (15 to 3111 rows, 3 to 3607 features), each timed on up to 64
+// slices of either product: the picks are within 3 % of the best in the mean, 14 % at worst (1419 rows, 74 -> 60);
+// 3111 rows of 121 -> 442 take 31 us on 14 and 2 slices, 108 whole and 44 on as many as the plain products take.
 // Returns the modelled time.
 double plan_act_slices(GemmParams* const* p, int count) {
   int nk[2] = {0, 0}, longest = 0;
@@ -1493,7 +1484,7 @@ double plan_act_slices(GemmParams* const* p, int count) {
     tiles[i] = (long long)((p[i]->M + 31) / 32) * ((p[i]->N + 31) / 32);
     if (nk[i] > longest) longest = nk[i];
   }
-  const double join = count > 1 ? 3.6 : 2.6;
+  const double join = count > 1 ? 3.7 : 2.6;
   int steps = longest;
   double best = 0.0;
   for (int j = 1; j <= 64; ++j) {
@@ -1501,14 +1492,17 @@ double plan_act_slices(GemmParams* const* p, int count) {
     if (j > 1 && n < 3) break;
     double work = 0.0, groups = 0.0;
     size_t need = 0;
+    int most = 1;
     for (int i = 0; i < count; ++i) {
       const int s = (nk[i] + n - 1) / n;
       work += (double)tiles[i] * nk[i];
       groups += (double)tiles[i] * s;
       if (s > 1) need += (size_t)s * ((size_t)p[i]->M * p[i]->N + (size_t)p[i]->M);
+      if (s > most) most = s;
     }
     if (j > 1 && need > room) break;
-    const double c = 3.7 + (0.14 * work + 0.59 * groups) / 256.0 + 0.35 * n + (j > 1 ? join : 0.0);
+    const double c = 3.8 + (0.12 * work + 0.65 * groups) / 256.0 + 0.35 * n +
+                     (j > 1 ? join + 1.8e-6 * (double)need + (most > 32 ? 2.1 : 0.0) : 0.0);
     if (j == 1 || c < best) {
       best = c;
       steps = n;
