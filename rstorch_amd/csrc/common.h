@@ -102,13 +102,13 @@ int launch_linear_rows(hipStream_t s, const double* x, const double* w, const do
 // sliced ones; same results as launch_gemm on each, except that from a batch of about 4096 a
 // group of weight gradients runs as K-sliced 128x128 tiles whose slices differ from a lone launch's
 // (equal within rounding, 1e-13).  The descriptors share one workspace, of which the group as a
-// whole takes gemm_group_workspace(d, count) doubles.  A member with an ActEpilogue: a weight gradient and the
-// layer's input gradient, which carries it.
+// whole takes gemm_group_workspace(d, count) doubles.
 bool can_group_gemm(const GemmDesc& d);
 size_t gemm_group_workspace(const GemmDesc* d, int count);
-bool can_group_grads_act(const GemmDesc* d);  // d[0] a weight gradient, d[1] the input gradient with an ActEpilogue
 int max_gemm_group();
 int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count);
+// A layer's weight gradient and its input gradient with an ActEpilogue in one grid, where that is the faster way: *taken
+int launch_grads_act(hipStream_t stream, const GemmDesc& weight_grad, const GemmDesc& input_grad, bool* taken);
 
 // ---- streaming kernels -----------------------------------------------------------------------
 int launch_relu_forward(hipStream_t s, const double* x, double* out, size_t n);

@@ -1155,19 +1155,26 @@ __global__ __launch_bounds__(WGM * WGN * 64, (BURST > 0 ? 1 : WGM * WGN >= 8 ? 4
   gemm_tile<BM, BN, WGM, WGN, true, B_KC, VEC, BURST>(p, (int)blockIdx.x, lds_a, lds_b, ActFinish<!B_KC>{e});
 }
 
-// A layer's weight gradient (member 0) and its input gradient with the epilogue (member 1) in one grid.
+// A layer's weight gradient (p[0], the first workgroups) and its input gradient with the epilogue (p[1]) in one grid.
+struct GradsPair {
+  int first_block, first_reduce_block;  // of the input gradient
+  GemmParams p[2];
+};
 template <int BURST>
-__global__ __launch_bounds__(256, (BURST > 0 ? 1 : 2)) void gemm_f64_mfma_grads_act(const GemmGroup g, const ActEpilogue e) {
+__global__ __launch_bounds__(256, (BURST > 0 ? 1 : 2)) void gemm_f64_mfma_grads_act(const GradsPair g, const ActEpilogue e) {
   __shared__ __attribute__((aligned(16))) double lds_a[tile_lds_doubles<32, false, 256, BURST>()];
   __shared__ __attribute__((aligned(16))) double lds_b[tile_lds_doubles<32, false, 256, BURST>()];
-  const int i = group_member_of_block(g.first_block, g.count, (int)blockIdx.x);
-  const int block = (int)blockIdx.x - g.first_block[i];
+  // (members named, not indexed: an indexed one is selected field by field)
+  const PlainFinish plain;
   const ActFinish<true> finish{e};
-  switch (2 * i + g.p[i].unaligned) {
-    case 0: gemm_tile<32, 32, 2, 2, false, false, true, BURST>(g.p[i], block, lds_a, lds_b); break;
-    case 1: gemm_tile<32, 32, 2, 2, false, false, false, BURST>(g.p[i], block, lds_a, lds_b); break;
-    case 2: gemm_tile<32, 32, 2, 2, true, false, true, BURST>(g.p[i], block, lds_a, lds_b, finish); break;
-    default: gemm_tile<32, 32, 2, 2, true, false, false, BURST>(g.p[i], block, lds_a, lds_b, finish); break;
+  if ((int)blockIdx.x < g.first_block) {
+    const int block = (int)blockIdx.x;
+    if (g.p[0].unaligned) gemm_tile<32, 32, 2, 2, false, false, false, BURST>(g.p[0], block, lds_a, lds_b, plain);
+    else gemm_tile<32, 32, 2, 2, false, false, true, BURST>(g.p[0], block, lds_a, lds_b, plain);
+  } else {
+    const int block = (int)blockIdx.x - g.first_block;
+    if (g.p[1].unaligned) gemm_tile<32, 32, 2, 2, true, false, false, BURST>(g.p[1], block, lds_a, lds_b, finish);
+    else gemm_tile<32, 32, 2, 2, true, false, true, BURST>(g.p[1], block, lds_a, lds_b, finish);
   }
 }
 
@@ -1322,11 +1329,9 @@ __global__ __launch_bounds__(256) void split_reduce_act_kernel(const GemmParams 
 }
 
 // (of gemm_f64_mfma_grads_act)
-__global__ __launch_bounds__(256) void split_reduce_grads_act_kernel(const GemmGroup g, const ActEpilogue e) {
-  const int i = group_member_of_block(g.first_reduce_block, g.count, (int)blockIdx.x);
-  const size_t block = (size_t)((int)blockIdx.x - g.first_reduce_block[i]);
-  if (i == 1) split_reduce_act_body<true>(g.p[1], e, block);
-  else split_reduce_body(g.p[0], block);
+__global__ __launch_bounds__(256) void split_reduce_grads_act_kernel(const GradsPair g, const ActEpilogue e) {
+  if ((int)blockIdx.x >= g.first_reduce_block) split_reduce_act_body<true>(g.p[1], e, blockIdx.x - g.first_reduce_block);
+  else split_reduce_body(g.p[0], blockIdx.x);
 }
 
 // e: the residual block's epilogue of a product whose B is (GRAD: output-) contraction-contiguous, or NULL
@@ -1487,7 +1492,7 @@ double plan_act_slices(GemmParams* const* p, int count) {
   const double join = count > 1 ? 3.7 : 2.6;
   int steps = longest;
   double best = 0.0;
-  for (int j = 1; j <= 64; ++j) {
+  for (int j = 1; j <= 64; j += 1 + j / 4) {
     const int n = (longest + j - 1) / j;
     if (j > 1 && n < 3) break;
     double work = 0.0, groups = 0.0;
@@ -1834,20 +1839,11 @@ int launch_gemm(hipStream_t stream, const GemmDesc& d) {
 int max_gemm_group() { return kMaxGroup; }
 
 namespace {
-// the parameters of a group of 32x32 tiles, its slices planned: what launch_gemm would choose for each member alone, or,
-// with the residual block's epilogue in the group, both by plan_act_slices
-void plan_group(const GemmDesc* d, int count, GemmParams* p) {
-  for (int i = 0; i < count; ++i) {
-    p[i] = make_params(d[i]);
-    p[i].tiles_m = (p[i].M + 31) / 32;
-    p[i].tiles_n = (p[i].N + 31) / 32;
-  }
-  if (count == 2 && d[1].act) {
-    GemmParams* const both[2] = {&p[0], &p[1]};
-    plan_act_slices(both, 2);
-    return;
-  }
-  for (int i = 0; i < count; ++i) plan_slices(p[i], (long long)p[i].tiles_m * p[i].tiles_n, kSmallTileSplitBelow, 2048);
+// the slices of a group member: what launch_gemm would choose for it alone
+void plan_group_member(GemmParams& p) {
+  p.tiles_m = (p.M + 31) / 32;
+  p.tiles_n = (p.N + 31) / 32;
+  plan_slices(p, (long long)p.tiles_m * p.tiles_n, kSmallTileSplitBelow, 2048);
 }
 }  // namespace
 
@@ -2012,11 +2008,11 @@ size_t gemm_group_workspace(const GemmDesc* d, int count) {
     if (plan_dma_group(d, count, &g, &blocks, &reduce_blocks, &need)) return need;
   }
   size_t need = 0;
-  if (count < 1 || count > kMaxGroup) return need;
-  GemmParams p[kMaxGroup];
-  plan_group(d, count, p);
-  for (int i = 0; i < count; ++i)
-    if (p[i].split_k > 1) need += (size_t)p[i].split_k * ((size_t)p[i].M * p[i].N + (size_t)p[i].M);
+  for (int i = 0; i < count; ++i) {
+    GemmParams p = make_params(d[i]);
+    plan_group_member(p);
+    if (p.split_k > 1) need += (size_t)p.split_k * ((size_t)p.M * p.N + (size_t)p.M);
+  }
   return need;
 }
 
@@ -2041,15 +2037,10 @@ int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count) {
   blocks = reduce_blocks = 0;
   size_t ws_used = 0;
   bool mixed = false;  // anything but weight-gradient layouts
-  const ActEpilogue* act = count == 2 ? d[1].act : nullptr;
-  if (act && (d[0].a_kc || d[0].b_kc || !d[1].a_kc || d[1].b_kc))
-    return fail(RST_ERR_INVALID_ARGUMENT, "an activation epilogue belongs to the input gradient behind a weight gradient");
-  GemmParams planned[kMaxGroup];
-  plan_group(d, count, planned);
   for (int i = 0; i < count; ++i) {
-    if (!(act ? d[i].M > 0 && d[i].N > 0 : can_group_gemm(d[i])) || (d[i].act && d[i].act != act))
-      return fail(RST_ERR_INVALID_ARGUMENT, "contraction %d cannot join a group", i);
-    GemmParams& p = planned[i];
+    if (!can_group_gemm(d[i])) return fail(RST_ERR_INVALID_ARGUMENT, "contraction %d cannot join a group", i);
+    GemmParams p = make_params(d[i]);
+    plan_group_member(p);
     g.first_block[i] = (int)blocks;
     g.first_reduce_block[i] = (int)reduce_blocks;
     g.layout[i] = (unsigned char)((d[i].a_kc ? 1 : 0) | (d[i].b_kc ? 2 : 0));
@@ -2071,12 +2062,8 @@ int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count) {
   g.first_reduce_block[count] = (int)reduce_blocks;
   const bool burst = blocks <= compute_units();
   RST_OBSERVE_GEMM(mixed ? GemmKernel::kStagedMixedGroup : GemmKernel::kStagedGroup, 32, 32, 2, 2, false, false, true,
-                   burst ? kBurst : 0, blocks, 256, nullptr, nullptr, 0, &g, act != nullptr);
-  if (act && burst)
-    hipLaunchKernelGGL(gemm_f64_mfma_grads_act<kBurst>, dim3((unsigned)blocks), dim3(256), 0, stream, g, *act);
-  else if (act)
-    hipLaunchKernelGGL(gemm_f64_mfma_grads_act<0>, dim3((unsigned)blocks), dim3(256), 0, stream, g, *act);
-  else if (mixed && burst)
+                   burst ? kBurst : 0, blocks, 256, nullptr, nullptr, 0, &g);
+  if (mixed && burst)
     hipLaunchKernelGGL((gemm_f64_mfma_mixed_group<kBurst>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
   else if (mixed)
     hipLaunchKernelGGL((gemm_f64_mfma_mixed_group<0>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
@@ -2086,37 +2073,98 @@ int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count) {
     hipLaunchKernelGGL((gemm_f64_mfma_group<false, false, 0>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
   RST_HIP(hipGetLastError());
   if (reduce_blocks > 0) {
-    RST_OBSERVE_GEMM(GemmKernel::kSplitReduceGroup, 0, 0, 0, 0, false, false, false, 0, reduce_blocks, 256, nullptr, nullptr, 0, &g, act != nullptr);
-    if (act)
-      hipLaunchKernelGGL(split_reduce_grads_act_kernel, dim3((unsigned)reduce_blocks), dim3(256), 0, stream, g, *act);
-    else
-      hipLaunchKernelGGL(split_reduce_group_kernel, dim3((unsigned)reduce_blocks), dim3(256), 0, stream, g);
+    RST_OBSERVE_GEMM(GemmKernel::kSplitReduceGroup, 0, 0, 0, 0, false, false, false, 0, reduce_blocks, 256, nullptr, nullptr, 0, &g);
+    hipLaunchKernelGGL(split_reduce_group_kernel, dim3((unsigned)reduce_blocks), dim3(256), 0, stream, g);
     RST_HIP(hipGetLastError());
   }
   return RST_OK;
 }
 
-// Both gradients of a layer in one grid of 32x32 tiles, or each on the tiles that suit it: whichever the two models
-// find shorter; the larger tiles from 3 GFLOP on.  On 46 layers of 0.25 to 10 GFLOP, each timed both ways, the pick is
-// within 1.3 % of the better in the mean, 10 % at worst: 1953 rows of 32 -> 3607 take 38 us together and 75 apart, 1462 of
-// 189 -> 529 29 and 38, 1024 of 1024 -> 1024 112 and 91.
-bool can_group_grads_act(const GemmDesc* d) {
-  if (!d[1].act || d[0].M <= 0 || d[0].N <= 0 || d[1].M <= 0 || d[1].N <= 0) return false;
-  if (4.0 * d[0].M * d[0].N * (double)d[0].K >= 3e9 || gemm_group_workspace(d, 2) > d[0].workspace_count) return false;
-  GemmParams p[2] = {make_params(d[0]), make_params(d[1])};
-  GemmParams* const both[2] = {&p[0], &p[1]};
-  const double together = plan_act_slices(both, 2);
-  double apart = 0.0;
+namespace {
+// The time that both gradients of a layer take on the tiles that suit each, by the models of plan_act and plan_act_slices.
+double grads_apart(const GemmParams* p) {
+  double sum = 0.0;
   for (int i = 0; i < 2; ++i) {
     int slices = 0;
     const Route route = choose_route(p[i], &slices, i == 1, false);
     const ActPlan plan = i == 1 ? plan_act(p[i], true, false) : ActPlan{0, 1};
-    if (route == Route::kTile128) return false;
-    if (route == Route::kTile32) apart += plan_act_slices(&both[i], 1);
-    else if (plan.tile != 0) apart += dma_cost(p[i], plan.tile, plan.slices);
-    else apart += dma_cost(p[i], route == Route::kDma64 ? 64 : 128, slices > 1 ? slices : 1);
+    GemmParams alone = p[i];
+    GemmParams* const self = &alone;
+    if (route == Route::kTile32 || route == Route::kTile128) sum += plan_act_slices(&self, 1);
+    else if (plan.tile != 0) sum += dma_cost(p[i], plan.tile, plan.slices);
+    else sum += dma_cost(p[i], route == Route::kDma64 ? 64 : 128, slices > 1 ? slices : 1);
   }
-  return together < apart;
+  return sum;
+}
+
+// (for the launch observer)
+GemmGroup group_of(const GradsPair& g, int blocks, int reduce_blocks) {
+  GemmGroup all{};
+  all.count = 2;
+  all.first_block[1] = g.first_block;
+  all.first_block[2] = blocks;
+  all.first_reduce_block[1] = g.first_reduce_block;
+  all.first_reduce_block[2] = reduce_blocks;
+  all.layout[1] = 1;
+  all.p[0] = g.p[0];
+  all.p[1] = g.p[1];
+  return all;
+}
+}  // namespace
+
+// Both gradients of a layer in one grid of 32x32 tiles, or each on the tiles that suit it: whichever the two models
+// find shorter; the larger tiles from 3 GFLOP on.  On 46 layers of 0.25 to 10 GFLOP, each timed both ways, the pick is
+// within 1.3 % of the better in the mean, 10 % at worst: 1953 rows of 32 -> 3607 take 38 us together and 75 apart, 1462 of
+// 189 -> 529 29 and 38, 1024 of 1024 -> 1024 112 and 91.
+int launch_grads_act(hipStream_t stream, const GemmDesc& weight_grad, const GemmDesc& input_grad, bool* taken) {
+  *taken = false;
+  const ActEpilogue* act = input_grad.act;
+  if (!act || weight_grad.M <= 0 || weight_grad.N <= 0 || input_grad.M <= 0 || input_grad.N <= 0 || weight_grad.a_kc ||
+      weight_grad.b_kc || !input_grad.a_kc || input_grad.b_kc || weight_grad.workspace != input_grad.workspace)
+    return fail(RST_ERR_INVALID_ARGUMENT, "not the two gradients of a layer");
+  if (4.0 * weight_grad.M * weight_grad.N * (double)weight_grad.K >= 3e9) return RST_OK;
+  GradsPair g;
+  g.p[0] = make_params(weight_grad);
+  g.p[1] = make_params(input_grad);
+  GemmParams* const both[2] = {&g.p[0], &g.p[1]};
+  const double together = plan_act_slices(both, 2);
+  // (none of the 46 below 1 GFLOP was faster apart)
+  if (4.0 * weight_grad.M * weight_grad.N * (double)weight_grad.K >= 1e8 && together >= grads_apart(g.p)) return RST_OK;
+  long long blocks = 0, reduce_blocks = 0;
+  size_t ws_used = 0;
+  for (int i = 0; i < 2; ++i) {
+    GemmParams& p = g.p[i];
+    p.tiles_m = (p.M + 31) / 32;
+    p.tiles_n = (p.N + 31) / 32;
+    if (i == 1) {
+      g.first_block = (int)blocks;
+      g.first_reduce_block = (int)reduce_blocks;
+    }
+    blocks += (long long)p.tiles_m * p.tiles_n * p.split_k;
+    if (p.split_k == 1) continue;
+    // each product has a region of its own in the workspace (plan_act_slices has kept to its size)
+    p.ws += ws_used;
+    p.ws_colsum = p.ws + (size_t)p.split_k * p.M * p.N;
+    ws_used += (size_t)p.split_k * ((size_t)p.M * p.N + (size_t)p.M);
+    reduce_blocks += (long long)(((size_t)p.M * p.N + 255) / 256);
+  }
+  if (ws_used > g.p[0].ws_capacity) return fail(RST_ERR_INVALID_ARGUMENT, "group workspace exhausted");
+  if (blocks > 0x7fffffffLL || reduce_blocks > 0x7fffffffLL) return fail(RST_ERR_UNSUPPORTED, "contraction grid too large");
+  *taken = true;
+  const bool burst = blocks <= compute_units();
+#ifdef RST_GEMM_LAUNCH_OBSERVER
+  const GemmGroup all = group_of(g, (int)blocks, (int)reduce_blocks);
+#endif
+  RST_OBSERVE_GEMM(GemmKernel::kStagedMixedGroup, 32, 32, 2, 2, false, false, true, burst ? kBurst : 0, blocks, 256, nullptr, nullptr, 0, &all, true);
+  if (burst) hipLaunchKernelGGL(gemm_f64_mfma_grads_act<kBurst>, dim3((unsigned)blocks), dim3(256), 0, stream, g, *act);
+  else hipLaunchKernelGGL(gemm_f64_mfma_grads_act<0>, dim3((unsigned)blocks), dim3(256), 0, stream, g, *act);
+  RST_HIP(hipGetLastError());
+  if (reduce_blocks > 0) {
+    RST_OBSERVE_GEMM(GemmKernel::kSplitReduceGroup, 0, 0, 0, 0, false, false, false, 0, reduce_blocks, 256, nullptr, nullptr, 0, &all, true);
+    hipLaunchKernelGGL(split_reduce_grads_act_kernel, dim3((unsigned)reduce_blocks), dim3(256), 0, stream, g, *act);
+    RST_HIP(hipGetLastError());
+  }
+  return RST_OK;
 }
 
 bool can_pair_gemm(const GemmDesc& input_grad, const GemmDesc& weight_grad) {

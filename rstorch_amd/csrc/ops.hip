@@ -121,14 +121,23 @@ int engine_linear_backward(rst_engine* e, const double* grad, const double* x, c
   dx.mask = relu_mask_source; dx.ldmask = (long)in_features;
   dx.act = input_act;
   dx.workspace = e->d_gemm_ws; dx.workspace_count = e->gemm_ws_count;
-  // two small products that do not depend on each other: one grid
-  const GemmDesc both[2] = {dw, dx};
-  if (grad_input && (input_act ? can_group_grads_act(both)
-                               : can_group_gemm(dw) && can_group_gemm(dx) && gemm_group_workspace(both, 2) <= e->gemm_ws_count)) {
-    RST_TRY(launch_gemm_group(e->stream, both, 2));
-  } else if (grad_input && can_pair_grads_act(dw, dx)) {
-    RST_TRY(launch_gemm_grads_act(e->stream, dw, dx));
-  } else {
+  // two products that do not depend on each other: one grid where that pays
+  bool taken = false;
+  if (grad_input && input_act) {
+    if (can_pair_grads_act(dw, dx)) {
+      RST_TRY(launch_gemm_grads_act(e->stream, dw, dx));
+      taken = true;
+    } else {
+      RST_TRY(launch_grads_act(e->stream, dw, dx, &taken));
+    }
+  } else if (grad_input && can_group_gemm(dw) && can_group_gemm(dx)) {
+    const GemmDesc both[2] = {dw, dx};
+    if (gemm_group_workspace(both, 2) <= e->gemm_ws_count) {
+      RST_TRY(launch_gemm_group(e->stream, both, 2));
+      taken = true;
+    }
+  }
+  if (!taken) {
     RST_TRY(launch_gemm(e->stream, dw));
     if (grad_input) RST_TRY(launch_gemm(e->stream, dx));
   }
