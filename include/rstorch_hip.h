@@ -169,7 +169,7 @@ int rst_activation_backward(rst_engine* engine, const double* grad, const double
 
 /* z = x[batch,in] . weight[out,in]^T + bias[1,out];  out[batch,out] = act(z) + residual[batch,out].
  * bias, residual: NULL for none.  pre_out[batch,out] receives z for the backward pass (NULL: not kept).
- * out may be residual itself; out and pre_out are no other operand. */
+ * out may be residual itself; out and pre_out are no other operand (RST_ERR_INVALID_ARGUMENT). */
 int rst_linear_act_forward(rst_engine* engine, const double* x, const double* weight,
                            const double* bias, const double* residual, double* pre_out, double* out,
                            size_t batch, size_t in_features, size_t out_features, int activation);
@@ -181,7 +181,9 @@ int rst_linear_act_forward(rst_engine* engine, const double* x, const double* we
  * input_activation is what produced x from input_pre[batch,in] (its backward pass, fused as
  * rst_linear_backward fuses ReLU's; RST_ACT_NONE: input_pre is not used) and residual_grad[batch,in],
  * NULL for none, is what reaches this layer's input past it.  With both, residual_grad is the gradient
- * with respect to input_pre.  grad_input may be input_pre or residual_grad itself. */
+ * with respect to input_pre.  grad_input may be input_pre or residual_grad itself, but not what both
+ * products read (x, weight, dz; RST_ERR_INVALID_ARGUMENT): a layer whose residual_grad is its grad
+ * works in place where dz lies apart from both. */
 int rst_linear_act_backward(rst_engine* engine, const double* grad, const double* pre, int activation,
                             double* grad_pre, const double* x, const double* weight,
                             double* grad_weight, double* grad_bias, double* grad_input,

@@ -97,6 +97,9 @@ int rst_linear_act_forward(rst_engine* e, const double* x, const double* weight,
   if (batch == 0 || out_features == 0) return RST_OK;
   if (!out || (in_features && (!x || !weight)))
     return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_forward: null operand");
+  // (other workgroups still read these)
+  if (out == x || out == weight || (pre_out && (pre_out == x || pre_out == weight || pre_out == residual || pre_out == out)))
+    return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_forward: an output over an operand");
   RST_TRY(check_dim("linear_act_forward", batch, "batch"));
   RST_TRY(check_dim("linear_act_forward", in_features, "in_features"));
   RST_TRY(check_dim("linear_act_forward", out_features, "out_features"));
@@ -131,6 +134,9 @@ int rst_linear_act_backward(rst_engine* e, const double* grad, const double* pre
     return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_backward: an activation needs pre and grad_pre");
   if (grad_input && input_activation != RST_ACT_NONE && !input_pre)
     return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_backward: an input activation needs input_pre");
+  // (both products read these while the input gradient is written)
+  if (grad_input && (grad_input == x || grad_input == weight || grad_input == (activation != RST_ACT_NONE ? grad_pre : grad)))
+    return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_backward: grad_input over x, weight or the products' gradient");
   RST_TRY(check_dim("linear_act_backward", batch, "batch"));
   RST_TRY(check_dim("linear_act_backward", in_features, "in_features"));
   RST_TRY(check_dim("linear_act_backward", out_features, "out_features"));

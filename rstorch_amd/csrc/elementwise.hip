@@ -27,7 +27,8 @@ unsigned blocks_for(size_t n) {
   return (unsigned)(blocks < kMaxBlocks ? blocks : kMaxBlocks);
 }
 
-// out = act(z) [+ residual]
+// out = act(z) [+ residual].  16384 x 4096: ReLU 160 us (6.7 TB/s, as a flat copy), SiLU 170, tanh GELU 173; GELU 194: its
+// normal tail takes as many vector instructions as the bytes take time.
 template <int ACT, bool RES>
 __global__ __launch_bounds__(kBlock) void act_forward_kernel(const double* z, const double* residual, double* out,
                                                              size_t n) {
@@ -46,7 +47,7 @@ __global__ __launch_bounds__(kBlock) void act_forward_kernel(const double* z, co
   });
 }
 
-// out = g * act'(z) [+ residual]; with ACT == NONE z is not read
+// out = g * act'(z) [+ residual]; with ACT == NONE z is not read.  16384 x 4096: 247 us (6.5 TB/s), GELU 274.
 template <int ACT, bool RES>
 __global__ __launch_bounds__(kBlock) void act_backward_kernel(const double* g, const double* z, const double* residual,
                                                               double* out, size_t n) {
@@ -70,7 +71,8 @@ __global__ __launch_bounds__(kBlock) void act_backward_kernel(const double* g, c
 
 // Dropout: element i is kept when the generator's value(seed, stream, i) >= p, i.e. when the top 53
 // bits of its word are at least ceil(p 2^53); the backward pass draws the same words again.  A dropped
-// element is 0 whatever x holds there (inf and NaN included).
+// element is 0 whatever x holds there (inf and NaN included).  A mask that is drawn again costs two 64-bit multiplies an
+// element and no bytes: 16384 x 4096 162 us (6.6 TB/s), 2047 x 4095 with a residual 32 us (6.2 TB/s).
 template <bool RES>
 __global__ __launch_bounds__(kBlock) void dropout_kernel(const double* x, const double* residual, double* out, size_t n,
                                                          uint64_t key, uint64_t threshold, double scale) {

@@ -7,6 +7,7 @@
 // of them in flight; a lane multiplies its pair of weights with the same pair of every x row (x is small and
 // stays in the caches).  The wavefronts of a workgroup share the length of the same weight rows; their sums
 // meet in LDS and are added in wavefront order, then the epilogue runs.
+// 4096 -> 4096 features: one row 23 us (5.8 TB/s; 30.5 on the tiles), eight rows 34 (42 on the tiles).
 #include "activation.h"
 #include "common.h"
 #include "vec.h"

@@ -43,6 +43,7 @@ int main() {
   rst_engine* e = nullptr;
   EXPECT(rst_engine_create(0, &e), RST_OK);
   double* const p = reinterpret_cast<double*>((uintptr_t)1 << 40);  // never dereferenced: kernels do not run
+  double *const q = p + ((size_t)1 << 36), *const r = q + ((size_t)1 << 36);
   double* const none = nullptr;
   const double nan = std::nan(""), inf = std::numeric_limits<double>::infinity();
   const size_t huge = (size_t)1 << 31;
@@ -94,9 +95,9 @@ int main() {
   for (int bad : {-1, 5, 1000}) {
     EXPECT(rst_activation_forward(e, p, p, p, 8, bad), INVALID);
     EXPECT(rst_activation_backward(e, p, p, p, p, 8, bad), INVALID);
-    EXPECT(rst_linear_act_forward(e, p, p, p, p, p, p, 8, 8, 8, bad), INVALID);
-    EXPECT(rst_linear_act_backward(e, p, p, bad, p, p, p, p, p, p, p, RST_ACT_NONE, p, 8, 8, 8), INVALID);
-    EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_NONE, p, p, p, p, p, p, p, bad, p, 8, 8, 8), INVALID);
+    EXPECT(rst_linear_act_forward(e, p, p, p, p, r, q, 8, 8, 8, bad), INVALID);
+    EXPECT(rst_linear_act_backward(e, p, p, bad, p, p, p, p, p, q, p, RST_ACT_NONE, p, 8, 8, 8), INVALID);
+    EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_NONE, p, p, p, p, p, q, p, bad, p, 8, 8, 8), INVALID);
   }
   EXPECT(rst_activation_forward(e, none, p, p, 8, RST_ACT_GELU), INVALID);
   EXPECT(rst_activation_forward(e, p, p, none, 8, RST_ACT_GELU), INVALID);
@@ -107,26 +108,41 @@ int main() {
   LAUNCHES(rst_activation_forward(e, none, none, none, 0, RST_ACT_RELU), 0);
 
   // Linear with activation and residual
-  EXPECT(rst_linear_act_forward(nullptr, p, p, p, p, p, p, 8, 8, 8, RST_ACT_GELU), INVALID);
-  EXPECT(rst_linear_act_forward(e, none, p, p, p, p, p, 8, 8, 8, RST_ACT_GELU), INVALID);
-  EXPECT(rst_linear_act_forward(e, p, none, p, p, p, p, 8, 8, 8, RST_ACT_GELU), INVALID);
-  EXPECT(rst_linear_act_forward(e, p, p, p, p, p, none, 8, 8, 8, RST_ACT_GELU), INVALID);
-  EXPECT(rst_linear_act_forward(e, p, p, p, p, p, p, huge, 8, 8, RST_ACT_GELU), UNSUPPORTED);
-  EXPECT(rst_linear_act_forward(e, p, p, p, p, p, p, 8, huge, 8, RST_ACT_GELU), UNSUPPORTED);
-  EXPECT(rst_linear_act_forward(e, p, p, p, p, p, p, 8, 8, huge, RST_ACT_GELU), UNSUPPORTED);
+  EXPECT(rst_linear_act_forward(nullptr, p, p, p, p, r, q, 8, 8, 8, RST_ACT_GELU), INVALID);
+  EXPECT(rst_linear_act_forward(e, none, p, p, p, r, q, 8, 8, 8, RST_ACT_GELU), INVALID);
+  EXPECT(rst_linear_act_forward(e, p, none, p, p, r, q, 8, 8, 8, RST_ACT_GELU), INVALID);
+  EXPECT(rst_linear_act_forward(e, p, p, p, p, r, none, 8, 8, 8, RST_ACT_GELU), INVALID);
+  EXPECT(rst_linear_act_forward(e, p, p, p, p, r, q, huge, 8, 8, RST_ACT_GELU), UNSUPPORTED);
+  EXPECT(rst_linear_act_forward(e, p, p, p, p, r, q, 8, huge, 8, RST_ACT_GELU), UNSUPPORTED);
+  EXPECT(rst_linear_act_forward(e, p, p, p, p, r, q, 8, 8, huge, RST_ACT_GELU), UNSUPPORTED);
+  // an output over an operand that is still read
+  EXPECT(rst_linear_act_forward(e, q, p, p, p, r, q, 8, 8, 8, RST_ACT_GELU), INVALID);
+  EXPECT(rst_linear_act_forward(e, p, q, p, p, r, q, 8, 8, 8, RST_ACT_GELU), INVALID);
+  EXPECT(rst_linear_act_forward(e, r, p, p, p, r, q, 8, 8, 8, RST_ACT_GELU), INVALID);
+  EXPECT(rst_linear_act_forward(e, p, r, p, p, r, q, 8, 8, 8, RST_ACT_GELU), INVALID);
+  EXPECT(rst_linear_act_forward(e, p, p, p, r, r, q, 8, 8, 8, RST_ACT_GELU), INVALID);
+  EXPECT(rst_linear_act_forward(e, p, p, p, p, q, q, 8, 8, 8, RST_ACT_GELU), INVALID);
+  EXPECT(rst_linear_act_forward(e, p, p, p, q, r, q, 8, 8, 8, RST_ACT_GELU), RST_OK);
   LAUNCHES(rst_linear_act_forward(e, none, none, none, none, none, none, 0, 8, 8, RST_ACT_GELU), 0);
-  EXPECT(rst_linear_act_backward(e, none, p, RST_ACT_GELU, p, p, p, p, p, p, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
-  EXPECT(rst_linear_act_backward(e, p, none, RST_ACT_GELU, p, p, p, p, p, p, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
-  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, none, p, p, p, p, p, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
-  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, none, p, p, p, p, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
-  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, none, p, p, p, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
-  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, none, p, p, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
-  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, p, p, p, none, RST_ACT_GELU, p, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, none, p, RST_ACT_GELU, p, p, p, p, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, p, none, RST_ACT_GELU, p, p, p, p, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, none, p, p, p, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, none, p, p, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, none, p, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, none, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, p, p, q, none, RST_ACT_GELU, p, 8, 8, 8), INVALID);
   for (int zero = 0; zero < 3; ++zero)
-    EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, p, p, p, p, RST_ACT_GELU, p, zero == 0 ? 0 : 8,
+    EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, p, p, q, p, RST_ACT_GELU, p, zero == 0 ? 0 : 8,
                                    zero == 1 ? 0 : 8, zero == 2 ? 0 : 8), SHAPE);
-  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, p, p, p, p, RST_ACT_GELU, p, huge, 8, 8), UNSUPPORTED);
+  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, p, p, q, p, RST_ACT_GELU, p, huge, 8, 8), UNSUPPORTED);
   EXPECT(rst_linear_act_backward(e, p, none, RST_ACT_NONE, none, p, p, p, none, none, none, RST_ACT_GELU, none, 8, 8, 8), RST_OK);
+  // grad_input over x, the weight, or the gradient that both products read
+  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, q, p, p, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, q, p, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, q, p, p, p, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, q, p, RST_ACT_GELU, q, p, p, p, p, q, p, RST_ACT_GELU, q, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, q, none, RST_ACT_NONE, none, p, p, p, p, q, none, RST_ACT_NONE, q, 8, 8, 8), INVALID);
+  EXPECT(rst_linear_act_backward(e, q, p, RST_ACT_GELU, p, p, p, p, p, q, p, RST_ACT_GELU, q, 8, 8, 8), RST_OK);
 
   // inside a stream capture, over the routes of the planner
   const long allocations = hip_stub_allocation_calls();
@@ -135,8 +151,8 @@ int main() {
     for (size_t k : {1u, 100u, 785u, 4096u})
       for (size_t n : {1u, 10u, 101u, 1024u, 4608u})
         for (int act = RST_ACT_NONE; act <= RST_ACT_SILU; ++act) {
-          EXPECT(rst_linear_act_forward(e, p, p, p, act & 1 ? p : none, act & 2 ? p : none, p, b, k, n, act), RST_OK);
-          EXPECT(rst_linear_act_backward(e, p, p, act, p, p, p, p, p, p, p, RST_ACT_SILU - act, act & 1 ? p : none, b, k, n), RST_OK);
+          EXPECT(rst_linear_act_forward(e, p, p, p, act & 1 ? p : none, act & 2 ? r : none, q, b, k, n, act), RST_OK);
+          EXPECT(rst_linear_act_backward(e, p, p, act, p, p, p, p, p, q, p, RST_ACT_SILU - act, act & 1 ? p : none, b, k, n), RST_OK);
         }
   EXPECT(rst_layer_norm_forward(e, p, p, p, p, p, p, 100, 1000, 1e-5), RST_OK);
   EXPECT(rst_layer_norm_backward(e, p, p, p, p, p, p, p, p, p, 100, 1000), RST_OK);
