@@ -124,7 +124,8 @@ int rst_softmax_backward(rst_engine* engine, const double* grad, const double* o
  *      (no counterpart in the reference; x + Dropout(Linear(act(Linear(LayerNorm(x))))) and its
  *      backward pass).  Parameter gradients are divided by the number of rows, as Linear's are
  *      (src/module/linear.rs:62-66), and overwritten, never accumulated.  Arrays need their 8-byte
- *      alignment only and have any extents.  Nothing here allocates or waits; launches recorded into
+ *      alignment only and have any extents up to 2^31 - 128 (layer norm's backward pass over rows of one value:
+ *      2^23 rows; more is RST_ERR_UNSUPPORTED).  Nothing here allocates or waits; launches recorded into
  *      a graph of the caller's use the engine's scratch as the eager ones do: graphs of one engine run
  *      one at a time, on its stream ------------------------------------------------------------------ */
 /* RST_ACT_GELU: z (1 + erf(z / sqrt 2)) / 2;  RST_ACT_GELU_TANH: z (1 + tanh(sqrt(2 / pi) (z +

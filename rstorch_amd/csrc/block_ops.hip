@@ -10,8 +10,10 @@ using namespace rst;
 
 namespace {
 
+// (the last tile's row and column numbers are ints too)
+constexpr size_t kMostExtent = (size_t)INT_MAX - 127;
 int check_dim(const char* who, size_t v, const char* what) {
-  if (v > (size_t)INT_MAX) return fail(RST_ERR_UNSUPPORTED, "%s: %s = %zu exceeds 2^31-1", who, what, v);
+  if (v > kMostExtent) return fail(RST_ERR_UNSUPPORTED, "%s: %s = %zu exceeds 2^31-128", who, what, v);
   return RST_OK;
 }
 

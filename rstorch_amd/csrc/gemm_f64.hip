@@ -1488,7 +1488,7 @@ void plan_slices(GemmParams& p, long long blocks, long long split_below, long lo
 // 3111 rows of 121 -> 442 take 31 us on 14 and 2 slices, 108 whole and 44 on as many as the plain products take.
 // Returns the modelled time.
 double plan_act_slices(GemmParams* const* p, int count) {
-  int nk[2] = {0, 0}, longest = 0;
+  int nk[2] = {0, 0}, longest = 1;  // (no contraction at all: one slice of nothing)
   long long tiles[2] = {0, 0};
   size_t room = p[0]->ws != nullptr ? p[0]->ws_capacity : 0;
   for (int i = 0; i < count; ++i) {

@@ -422,8 +422,8 @@ __global__ __launch_bounds__(BLOCK, WAVES) void norm_backward_kernel(const NormG
 }
 
 // out[c] = (sum over the workgroups, in order, of partial[block][c]) / rows, c in [0, 2 cols): the
-// weight's columns, then the bias's.  5 us behind 8192 x 4096 (256 sets of 8192 sums).  16 columns x 16 parts of the workgroups per launch workgroup; the
-// parts are added in order.
+// weight's columns, then the bias's.  5 us behind 8192 x 4096 (256 sets of 8192 sums).  16 columns x 16 parts of the
+// workgroups per launch workgroup; the parts are added in order.
 __global__ __launch_bounds__(256) void norm_columns_kernel(const double* __restrict__ partial, double* grad_weight,
                                                            double* grad_bias, size_t cols, int blocks, double rows) {
   __shared__ double part[16][17];

@@ -2,6 +2,7 @@
 // every refusal comes back as its status before anything is launched, and every accepted shape gets
 // through the planners (kernels do not run).  The stand-in aborts on an allocation or a synchronisation
 // during stream capture, which covers "nothing here allocates or waits".
+#include <climits>
 #include <cmath>
 #include <cstdio>
 #include <cstdint>
@@ -87,6 +88,8 @@ int main() {
   EXPECT(rst_dropout_forward(e, p, p, none, 8, 0.5, 1, 2), INVALID);
   EXPECT(rst_dropout_backward(e, none, p, 8, 0.5, 1, 2), INVALID);
   EXPECT(rst_dropout_backward(e, p, none, 8, 0.5, 1, 2), INVALID);
+  EXPECT(rst_layer_norm_backward(e, p, p, p, p, p, none, p, p, p, ((size_t)1 << 23) + 1, 1), UNSUPPORTED);
+  EXPECT(rst_layer_norm_backward(e, p, p, p, p, p, none, p, p, p, (size_t)1 << 23, 1), RST_OK);
   LAUNCHES(rst_dropout_forward(e, none, none, none, 0, 0.5, 1, 2), 0);
   LAUNCHES(rst_dropout_forward(e, p, none, p, 1, 0.0, 1, 2), 1);
   LAUNCHES(rst_dropout_backward(e, p, p, (size_t)1 << 36, std::nextafter(1.0, 0.0), 1, 2), 1);
@@ -115,6 +118,16 @@ int main() {
   EXPECT(rst_linear_act_forward(e, p, p, p, p, r, q, huge, 8, 8, RST_ACT_GELU), UNSUPPORTED);
   EXPECT(rst_linear_act_forward(e, p, p, p, p, r, q, 8, huge, 8, RST_ACT_GELU), UNSUPPORTED);
   EXPECT(rst_linear_act_forward(e, p, p, p, p, r, q, 8, 8, huge, RST_ACT_GELU), UNSUPPORTED);
+  // no features in: out = act(bias) + residual, nothing to multiply
+  LAUNCHES(rst_linear_act_forward(e, none, none, p, p, r, q, 8, 0, 8, RST_ACT_GELU), 1);
+  LAUNCHES(rst_linear_act_forward(e, none, none, p, p, r, q, 2, 0, 8, RST_ACT_GELU), 1);
+  // the tiles' row and column numbers stay below 2^31
+  for (size_t most : {(size_t)INT_MAX, (size_t)INT_MAX - 126}) {
+    EXPECT(rst_linear_act_forward(e, p, p, p, p, r, q, most, 1, 1, RST_ACT_GELU), UNSUPPORTED);
+    EXPECT(rst_linear_act_forward(e, p, p, p, p, r, q, 1, 1, most, RST_ACT_GELU), UNSUPPORTED);
+    EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, p, p, q, p, RST_ACT_GELU, p, 1, most, 1), UNSUPPORTED);
+    EXPECT(rst_layer_norm_forward(e, p, p, p, p, p, p, most, 2, 0.1), UNSUPPORTED);
+  }
   // an output over an operand that is still read
   EXPECT(rst_linear_act_forward(e, q, p, p, p, r, q, 8, 8, 8, RST_ACT_GELU), INVALID);
   EXPECT(rst_linear_act_forward(e, p, q, p, p, r, q, 8, 8, 8, RST_ACT_GELU), INVALID);

@@ -224,3 +224,17 @@ def test_special_values_stay_in_their_row(engine):
         rest = [i for i in range(batch) if i != batch // 2]
         assert np.isnan(got[0][batch // 2]).all() and np.isnan(got[1][batch // 2]).all()
         assert np.array_equal(got[0][rest], clean[0][rest]) and np.array_equal(got[1][rest], clean[1][rest])
+
+
+@pytest.mark.parametrize("batch", (1, 3, 40, 300))
+def test_no_features_in(engine, batch):
+    """Nothing to multiply: out = act(bias) + residual, z = bias."""
+    rng = np.random.default_rng(batch)
+    b, res = rng.standard_normal((1, 90)), rng.standard_normal((batch, 90))
+    db, dres, out, pre = guarded(engine, b), guarded(engine, res), blank(engine, (batch, 90)), blank(engine, (batch, 90))
+    check(engine.lib.rst_linear_act_forward(engine.handle, None, None, db.ptr, dres.ptr, pre.ptr, out.ptr, batch, 0, 90,
+                                            ACTIVATIONS["silu"]))
+    z = np.broadcast_to(b, (batch, 90))
+    assert np.array_equal(pre.get(), z)
+    want = act(z, "silu")[0] + res
+    within(out.get(), want, act_bound(z) + 2 * U * np.abs(want), "act(bias) + residual")
