@@ -284,7 +284,7 @@ struct PlainFinish {
 // The residual block's epilogue (ActEpilogue): what an element needs from memory is requested for a fragment
 // row at a time, from clamped addresses, and only the stores are predicated (as in store_block).  Its vector time, some 75
 // instructions a value for GELU, is what the launch is longer than a plain product: 2048 x 1024 -> 4096 with GELU and z kept
-// 256 us (67 TFLOP/s), both gradients of 4096 -> 1024 at 2048 rows 493 us (70 TFLOP/s; a library product of 4096 reaches 76).
+// 256 us (67 TFLOP/s), both gradients of 4096 -> 1024 at 2048 rows 493 us (70 TFLOP/s; a library product of 8192 reaches 76).
 template <int TM, int TN, int ACT, bool GRAD>
 __device__ __forceinline__ void store_block_act(const GemmParams& p, const ActEpilogue& e, const v4d* acc, int row0,
                                                 int col0, int lr, int lk) {
