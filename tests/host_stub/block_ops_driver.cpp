@@ -167,6 +167,10 @@ int main() {
           EXPECT(rst_linear_act_forward(e, p, p, p, act & 1 ? p : none, act & 2 ? r : none, q, b, k, n, act), RST_OK);
           EXPECT(rst_linear_act_backward(e, p, p, act, p, p, p, p, p, q, p, RST_ACT_SILU - act, act & 1 ? p : none, b, k, n), RST_OK);
         }
+  // slices of one gradient, of the other, of both, in the shared grid
+  const size_t shared[][3] = {{1157, 233, 203}, {46, 2607, 939}, {518, 3, 2177}, {1953, 32, 3607}, {314, 1467, 790}, {2500, 20, 20}};
+  for (auto& d : shared)
+    EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, p, p, q, p, RST_ACT_GELU, p, d[0], d[1], d[2]), RST_OK);
   EXPECT(rst_layer_norm_forward(e, p, p, p, p, p, p, 100, 1000, 1e-5), RST_OK);
   EXPECT(rst_layer_norm_backward(e, p, p, p, p, p, p, p, p, p, 100, 1000), RST_OK);
   EXPECT(rst_dropout_forward(e, p, p, p, 100, 0.5, 1, 2), RST_OK);

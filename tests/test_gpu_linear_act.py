@@ -15,7 +15,8 @@ pytestmark = pytest.mark.gpu
 SHAPES = [(1, 1, 1), (1, 5, 3), (1, 784, 100), (1, 4096, 1000), (2, 257, 513), (3, 4095, 129), (4, 1024, 1024), (5, 100, 7),
           (8, 2048, 260), (9, 130, 31), (16, 512, 512), (17, 63, 65), (32, 784, 100), (33, 785, 101), (64, 1, 200),
           (100, 300, 33), (129, 17, 130), (512, 256, 384), (1024, 1024, 512), (2048, 100, 10), (1023, 1025, 511),
-          (512, 2048, 4096), (2050, 64, 2046), (2047, 1023, 1025), (2064, 2048, 2046), (1024, 2048, 4608), (8192, 100, 100)]
+          (512, 2048, 4096), (2050, 64, 2046), (2047, 1023, 1025), (2064, 2048, 2046), (1024, 2048, 4608), (8192, 100, 100),
+          (1157, 233, 203), (46, 2607, 939), (518, 3, 2177), (1953, 32, 3607), (314, 1467, 790)]
 KINDS = list(ACTIVATIONS)
 
 
