@@ -211,6 +211,10 @@ class SiLU(_Activation):
     kind = _ffi.ACT_SILU
 
 
+# the layers that a neighbouring Linear can take into its launches
+_FUSED = (ReLU, GELU, SiLU)
+
+
 class Dropout(Module):
     """In training (the state a module starts in; ``train`` / ``eval`` switch) zeroes each element with
     probability ``p`` and scales the others by 1 / (1 - p); in evaluation hands its input through.  No
@@ -694,15 +698,17 @@ class Sequential(Module):
                 width = layer._output_size(width)
         return width
 
+    # (exact types, here and where a Linear takes its neighbour's work: a subclass may override forward or
+    # backward, and is called like any other layer)
     def _next_real(self, i):
         for j in range(i + 1, len(self.layers)):
-            if not isinstance(self.layers[j], Identity):
+            if type(self.layers[j]) is not Identity:
                 return j
         return -1
 
     def _prev_real(self, i):
         for j in range(i - 1, -1, -1):
-            if not isinstance(self.layers[j], Identity):
+            if type(self.layers[j]) is not Identity:
                 return j
         return -1
 
@@ -728,8 +734,8 @@ class Sequential(Module):
                     behind._absorb_forward(x)
                     skip.add(j)
                     continue
-                if isinstance(behind, _Activation) or type(behind) is ReLU:
-                    kind = behind.kind if isinstance(behind, _Activation) else _ffi.ACT_RELU
+                if type(behind) in _FUSED:
+                    kind = _ffi.ACT_RELU if type(behind) is ReLU else behind.kind
                     x, pre = layer._forward_act(x, kind, residual if j == last else None)
                     behind._absorb_forward(pre)
                     skip.add(j)
@@ -768,8 +774,8 @@ class Sequential(Module):
                     before._absorb_backward()
                     skip.add(j)
                     continue
-                if (isinstance(before, _Activation) or type(before) is ReLU) and before.prev_input is not None:
-                    kind = before.kind if isinstance(before, _Activation) else _ffi.ACT_RELU
+                if type(before) in _FUSED and before.prev_input is not None:
+                    kind = _ffi.ACT_RELU if type(before) is ReLU else before.kind
                     g = layer._backward_act(g, before.prev_input, kind, residual if j == first else None)
                     before._absorb_backward()
                     skip.add(j)
@@ -812,7 +818,7 @@ class Residual(Module):
     the first one a Linear or LayerNorm."""
 
     def __init__(self, inner):
-        if isinstance(inner, Sequential):
+        if type(inner) is Sequential:  # (a subclass is a layer like any other: its own passes are called)
             self.inner = inner
         else:
             self.inner = Sequential(list(inner) if isinstance(inner, (list, tuple)) else [inner])

@@ -1,0 +1,139 @@
+"""Which calls the Python layers make, without a GPU: an engine that records the library's entry points instead of
+calling them, under Sequential and Residual."""
+import pytest
+
+import rstorch_amd as rs
+
+
+class Recorder:
+    """Stands for an Engine: hands out addresses and notes the entry points by name."""
+
+    device = 0
+
+    def __init__(self):
+        self.calls, self.handle, self._next = [], 1, 4096
+        recorder = self
+
+        class Lib:
+            def __getattr__(self, name):
+                def call(*args):
+                    recorder.calls.append(name)
+                    return 0
+                return call
+
+        self.lib = Lib()
+
+    def malloc(self, count):
+        self._next += 8 * int(count) + 4096
+        return self._next
+
+    def free(self, ptr):
+        pass
+
+    def empty(self, rows, cols):
+        return rs.Array2(self, rows, cols)
+
+    zeros = empty
+
+    def full(self, rows, cols, value):
+        return self.empty(rows, cols)
+
+    def normal(self, rows, cols, *args):
+        return self.empty(rows, cols)
+
+    def from_numpy(self, host):
+        return self.empty(*host.shape)
+
+    def taken(self):
+        calls, self.calls = self.calls, []
+        return calls
+
+
+@pytest.fixture
+def recorder():
+    return Recorder()
+
+
+def overridden(base):
+    """A subclass with passes of its own, which note that they ran."""
+
+    class Own(base):
+        def __init__(self, *args, **kw):
+            super().__init__(*args, **kw)
+            self.ran = []
+
+        def forward(self, input):
+            self.ran.append("forward")
+            return super().forward(input)
+
+        def backward(self, gradient):
+            self.ran.append("backward")
+            return super().backward(gradient)
+
+    return Own
+
+
+def neighbours(recorder, layer, where):
+    lin = lambda: rs.Linear(6, 6, engine=recorder)
+    return {"behind": [lin(), layer], "between": [lin(), layer, lin()], "in front": [layer, lin()],
+            "between a Linear and its activation": [lin(), layer, rs.GELU()],
+            "between an activation and a Linear": [rs.GELU(), layer, lin()]}[where]
+
+
+WHERE = ["behind", "between", "in front", "between a Linear and its activation", "between an activation and a Linear"]
+
+
+@pytest.mark.parametrize("where", WHERE)
+@pytest.mark.parametrize("base", [rs.GELU, rs.SiLU, rs.ReLU, rs.Dropout, rs.Identity])
+@pytest.mark.parametrize("outer", [rs.Sequential, rs.Residual])
+def test_an_overridden_layer_is_called(recorder, base, where, outer):
+    layer = overridden(base)()
+    model = outer(neighbours(recorder, layer, where))
+    x = recorder.empty(4, 6)
+    model.forward(x)
+    assert layer.ran == ["forward"]
+    model.backward(recorder.empty(4, 6))
+    assert layer.ran == ["forward", "backward"]
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_an_overridden_norm_is_called(recorder, first):
+    layer = overridden(rs.LayerNorm)(6, engine=recorder)
+    inner = [layer, rs.Linear(6, 6, engine=recorder)]
+    model = rs.Residual(inner if first else inner[::-1])
+    model.forward(recorder.empty(4, 6))
+    model.backward(recorder.empty(4, 6))
+    assert layer.ran == ["forward", "backward"]
+
+
+def test_an_overridden_sequential_is_called(recorder):
+    inner = overridden(rs.Sequential)([rs.Linear(6, 6, engine=recorder), rs.GELU()])
+    for model in (rs.Residual(inner), rs.Residual([inner]), rs.Sequential([inner])):
+        model.forward(recorder.empty(4, 6))
+        model.backward(recorder.empty(4, 6))
+        assert inner.ran == ["forward", "backward"]
+        inner.ran = []
+
+
+@pytest.mark.parametrize("kind", ["gelu", "relu"])
+def test_an_overridden_identity_keeps_its_place(recorder, kind):
+    """What it is given lies in front of the activation behind it."""
+    act = {"gelu": rs.GELU, "relu": rs.ReLU}[kind]()
+    name = {"gelu": "rst_activation_", "relu": "rst_relu_"}[kind]
+    model = rs.Sequential([rs.Linear(6, 6, engine=recorder), overridden(rs.Identity)(), act, overridden(rs.Identity)(),
+                           rs.Linear(6, 6, engine=recorder)])
+    recorder.taken()
+    model.forward(recorder.empty(4, 6))
+    assert recorder.taken() == ["rst_linear_forward", name + "forward", "rst_linear_forward"]
+    model.backward(recorder.empty(4, 6))
+    assert recorder.taken() == ["rst_linear_backward", name + "backward", "rst_linear_backward"]
+
+
+def test_a_linear_takes_its_neighbours_work(recorder):
+    """The layers themselves (not subclasses) stay joined."""
+    model = rs.Residual([rs.Linear(6, 9, engine=recorder), rs.GELU(), rs.Identity(), rs.Linear(9, 6, engine=recorder)])
+    recorder.taken()
+    model.forward(recorder.empty(4, 6))
+    assert recorder.taken() == ["rst_linear_act_forward"] * 2
+    model.backward(recorder.empty(4, 6))
+    assert recorder.taken() == ["rst_linear_act_backward"] * 2
