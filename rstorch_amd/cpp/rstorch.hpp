@@ -30,6 +30,7 @@
 #include <random>
 #include <stdexcept>
 #include <string>
+#include <typeinfo>
 #include <utility>
 #include <vector>
 
@@ -254,9 +255,18 @@ class Module {
   virtual void train() {}
   virtual void eval() {}
   virtual std::string debug() const = 0;  // the reference requires Debug of Sequential's layers
-  // Defaulted hooks that let Sequential fuse a Linear with the ReLU next to it.
+  // Defaulted hook that lets Sequential compile Identity, Linear and ReLU (not their subclasses, whatever they return).
   virtual int layer_kind() const { return -1; }
 };
+
+namespace detail {
+// m itself where it is an L and not a subclass of it (which may override forward or backward, and is called
+// like any other layer), else NULL
+template <class L>
+inline L* exactly(Module* m) {
+  return m && typeid(*m) == typeid(L) ? static_cast<L*>(m) : nullptr;
+}
+}  // namespace detail
 
 // ---- initialisers: src/module/init/{mod,he,xavier,sigma}.rs ------------------------------------
 class InitParameters {
@@ -652,6 +662,19 @@ class Linear : public Module {
 // ---- the compiled form of a Sequential of Identity / Linear / ReLU ------------------------------
 namespace detail {
 
+// RST_LAYER_* of the layers a compiled form holds, -1 for any other (their subclasses among them)
+inline int compiled_kind(Module* m) {
+  const int kind = m->layer_kind();
+  if (kind == RST_LAYER_LINEAR) return exactly<Linear>(m) ? kind : -1;
+  if (kind == RST_LAYER_RELU) return exactly<ReLU>(m) ? kind : -1;
+  return kind == RST_LAYER_IDENTITY && exactly<Identity>(m) ? kind : -1;
+}
+// the activations that a neighbouring Linear can take into its launches
+inline Activation* fused_activation(Module* m) {
+  if (auto* gelu = exactly<GELU>(m)) return gelu;
+  return exactly<SiLU>(m);
+}
+
 class Plan : public std::enable_shared_from_this<Plan> {
  public:
   // which object `home` tokens of this plan point at
@@ -746,8 +769,8 @@ class Plan : public std::enable_shared_from_this<Plan> {
     std::vector<size_t> in, out;
     for (auto& l : layers) {
       key_.push_back(l.get());
-      kinds.push_back(l->layer_kind());
-      Linear* lin = l->layer_kind() == RST_LAYER_LINEAR ? static_cast<Linear*>(l.get()) : nullptr;
+      kinds.push_back(compiled_kind(l.get()));
+      Linear* lin = exactly<Linear>(l.get());
       in.push_back(lin ? lin->input_size() : 0);
       out.push_back(lin ? lin->output_size() : 0);
       if (lin) linears_.push_back(lin);
@@ -875,22 +898,21 @@ class Sequential : public Module {
     const int last = prev_real(n);  // (-1: nothing but Identity)
     for (int i = 0; i < n; ++i) {
       Module* l = layers_[i].get();
-      if (l->layer_kind() == RST_LAYER_LINEAR) {
-        auto* linear = static_cast<Linear*>(l);
+      if (auto* linear = detail::exactly<Linear>(l)) {
         int j = next_real(i);
         Module* behind = j >= 0 ? layers_[j].get() : nullptr;
-        const bool relu = behind && behind->layer_kind() == RST_LAYER_RELU;
-        auto* act = dynamic_cast<Activation*>(behind);
+        auto* relu = detail::exactly<ReLU>(behind);
+        auto* act = detail::fused_activation(behind);
         const Array2* added = j == last ? residual : nullptr;
         if (act || relu) {
           if (relu && !added) {
             input = linear->forward_impl(std::move(input), true);
-            static_cast<ReLU*>(behind)->absorb_forward(input);
+            relu->absorb_forward(input);
           } else {
             Array2 pre;
             input = linear->forward_act(std::move(input), act ? act->kind() : RST_ACT_RELU, added, &pre);
             if (act) act->absorb_forward(std::move(pre));
-            else static_cast<ReLU*>(behind)->absorb_forward(pre);
+            else relu->absorb_forward(pre);
           }
           if (added) residual = nullptr;
           // Identity layers between the two pass the handle through; the activation is done
@@ -905,7 +927,7 @@ class Sequential : public Module {
         }
       }
       if (residual && i == last) {
-        if (auto* dropout = dynamic_cast<Dropout*>(l)) {
+        if (auto* dropout = detail::exactly<Dropout>(l)) {
           input = dropout->forward_impl(std::move(input), residual);
           residual = nullptr;
           continue;
@@ -926,13 +948,12 @@ class Sequential : public Module {
     const int first = next_real(-1);
     for (int i = n - 1; i >= 0; --i) {
       Module* l = layers_[i].get();
-      if (l->layer_kind() == RST_LAYER_LINEAR) {
-        auto* linear = static_cast<Linear*>(l);
+      if (auto* linear = detail::exactly<Linear>(l)) {
         int j = prev_real(i);
         Module* before = j >= 0 ? layers_[j].get() : nullptr;
-        auto* relu = before && before->layer_kind() == RST_LAYER_RELU ? static_cast<ReLU*>(before) : nullptr;
+        auto* relu = detail::exactly<ReLU>(before);
         if (relu && !relu->has_cache()) relu = nullptr;
-        auto* act = dynamic_cast<Activation*>(before);
+        auto* act = detail::fused_activation(before);
         if (act && !act->has_cache()) act = nullptr;
         const Array2* added = j == first ? residual : nullptr;
         if (act || relu) {
@@ -958,7 +979,7 @@ class Sequential : public Module {
         }
       }
       if (residual && i == first) {
-        if (auto* norm = dynamic_cast<LayerNorm*>(l)) {
+        if (auto* norm = detail::exactly<LayerNorm>(l)) {
           gradient = norm->backward_impl(std::move(gradient), residual);
           residual = nullptr;
           continue;
@@ -990,10 +1011,8 @@ class Sequential : public Module {
     size_t width = 0;
     bool any = false;
     for (auto& l : layers_) {
-      const int kind = l->layer_kind();
-      if (kind != RST_LAYER_IDENTITY && kind != RST_LAYER_RELU && kind != RST_LAYER_LINEAR) return nullptr;
-      if (kind == RST_LAYER_LINEAR) {
-        auto* lin = static_cast<Linear*>(l.get());
+      if (detail::compiled_kind(l.get()) < 0) return nullptr;
+      if (auto* lin = detail::exactly<Linear>(l.get())) {
         // (a width mismatch is left to the layer-by-layer pass, which panics where the reference does)
         if (any && lin->input_size() != width) return nullptr;
         width = lin->output_size();
@@ -1013,12 +1032,12 @@ class Sequential : public Module {
 
   int next_real(int i) const {
     for (int j = i + 1; j < int(layers_.size()); ++j)
-      if (layers_[j]->layer_kind() != RST_LAYER_IDENTITY) return j;
+      if (!detail::exactly<Identity>(layers_[j].get())) return j;
     return -1;
   }
   int prev_real(int i) const {
     for (int j = i - 1; j >= 0; --j)
-      if (layers_[j]->layer_kind() != RST_LAYER_IDENTITY) return j;
+      if (!detail::exactly<Identity>(layers_[j].get())) return j;
     return -1;
   }
   std::vector<std::unique_ptr<Module>> layers_;

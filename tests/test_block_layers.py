@@ -1,8 +1,15 @@
-"""Which calls the Python layers make, without a GPU: an engine that records the library's entry points instead of
-calling them, under Sequential and Residual."""
+"""Which calls the layers make, without a GPU: an engine that records the library's entry points instead of calling
+them, under the Python Sequential and Residual; the C++ ones over a stand-in HIP runtime
+(tests/host_stub/mirror_layers_driver.cpp)."""
+import os
+import shutil
+import subprocess
+
 import pytest
 
 import rstorch_amd as rs
+
+HOST = os.path.join(os.path.dirname(os.path.abspath(__file__)), "host_stub")
 
 
 class Recorder:
@@ -137,3 +144,12 @@ def test_a_linear_takes_its_neighbours_work(recorder):
     assert recorder.taken() == ["rst_linear_act_forward"] * 2
     model.backward(recorder.empty(4, 6))
     assert recorder.taken() == ["rst_linear_act_backward"] * 2
+
+
+@pytest.mark.skipif(shutil.which("hipcc") is None and not os.path.exists("/opt/rocm/bin/hipcc"),
+                    reason="needs hipcc to compile the host side")
+def test_layers_of_the_cpp_mirror():
+    build = subprocess.run(["make", "-C", HOST, "-j8", "-s"], capture_output=True, text=True)
+    assert build.returncode == 0, build.stderr[-3000:]
+    run = subprocess.run([os.path.join(HOST, "build", "mirror_layers_driver")], capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and "mirror layers ok" in run.stdout, (run.stdout + run.stderr)[-3000:]
