@@ -690,12 +690,15 @@ class Sequential(Module):
         return self.layers.pop(index)
 
     def _output_size(self, width):
-        """Columns of what the layers return for an input of ``width`` columns."""
+        """Columns of what the layers return for an input of ``width`` columns; None where a layer of the caller's own
+        decides that."""
         for layer in self.layers:
             if type(layer) is Linear:
                 width = layer.output_size
-            elif isinstance(layer, Sequential):
+            elif type(layer) is Sequential:
                 width = layer._output_size(width)
+            elif type(layer) not in _SAME_WIDTH:
+                width = None
         return width
 
     # (exact types, here and where a Linear takes its neighbour's work: a subclass may override forward or
@@ -832,7 +835,7 @@ class Residual(Module):
         x = as_array2(input)
         self.inner._drop_plan()  # (a compiled form would add in a pass of its own)
         wide = self.inner._output_size(x.cols)
-        if wide != x.cols:
+        if wide is not None and wide != x.cols:
             raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "a residual of %d features around layers that return %d"
                                   % (x.cols, wide))
         out = self.inner._layers_forward(x, x)
@@ -859,6 +862,10 @@ class Residual(Module):
 
     def __repr__(self):
         return "Residual(%s)" % ", ".join(repr(l) for l in self.inner.layers)
+
+
+# layers that return as many columns as they are given
+_SAME_WIDTH = (Identity, ReLU, Softmax, GELU, SiLU, Dropout, LayerNorm, Residual)
 
 
 def sequential(*layers):

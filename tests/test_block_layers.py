@@ -146,6 +146,35 @@ def test_a_linear_takes_its_neighbours_work(recorder):
     assert recorder.taken() == ["rst_linear_act_backward"] * 2
 
 
+class Resize(rs.Module):
+    """A layer of the caller's own that returns another width than it is given."""
+
+    def __init__(self, size):
+        self.size = size
+
+    def forward(self, input):
+        self.given = input.cols
+        return input.engine.empty(input.rows, self.size)
+
+    def backward(self, gradient):
+        return gradient.engine.empty(gradient.rows, self.given)
+
+
+def test_a_residual_around_layers_that_change_the_width(recorder):
+    lin = lambda k, n: rs.Linear(k, n, engine=recorder)
+    for inner in ([lin(6, 9), Resize(6)], [Resize(9), lin(9, 6)], [lin(6, 9), Resize(5), lin(5, 7), Resize(6)],
+                  [rs.Sequential([lin(6, 9), Resize(6)])], [lin(6, 9), Resize(6), rs.Dropout(0.5)]):
+        model = rs.Residual(inner)
+        assert model.forward(recorder.empty(4, 6)).shape == (4, 6)
+        assert model.backward(recorder.empty(4, 6)).shape == (4, 6)
+    # what does not fit is still refused; where the layers tell their width, before any of them runs
+    for inner in ([lin(6, 9)], [Resize(6), lin(6, 9)], [Resize(9)], [lin(6, 9), Resize(8)], [lin(6, 9), Resize(8), rs.Dropout(0.5)]):
+        recorder.taken()
+        with pytest.raises(rs.ShapeError):
+            rs.Residual(inner).forward(recorder.empty(4, 6))
+        assert not recorder.taken() or isinstance(inner[1], Resize)
+
+
 @pytest.mark.skipif(shutil.which("hipcc") is None and not os.path.exists("/opt/rocm/bin/hipcc"),
                     reason="needs hipcc to compile the host side")
 def test_layers_of_the_cpp_mirror():
