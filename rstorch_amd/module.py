@@ -227,7 +227,7 @@ class Dropout(Module):
         self.p, self.seed = float(p), _fresh_seed() if seed is None else int(seed) & 0xFFFFFFFFFFFFFFFF
         self.training = True
         self._calls = 0
-        self._kept = None  # (shape, stream) of the last forward; stream None: handed through
+        self._kept = None  # (shape, engine, stream) of the last forward; stream None: handed through
 
     @classmethod
     def new(cls, p):
@@ -243,13 +243,13 @@ class Dropout(Module):
         x = as_array2(input)
         _same_shape(residual, x.shape)
         if not self.training or self.p == 0.0:
-            self._kept = (x.shape, None)
+            self._kept = (x.shape, x.engine, None)
             return x if residual is None else _add(x, residual)
         stream, self._calls = self._calls, self._calls + 1
         out = x.engine.empty(x.rows, x.cols)
         _ffi.check(x.engine.lib.rst_dropout_forward(x.engine.handle, x.ptr, residual.ptr if residual else None,
                                                     out.ptr, x.size, self.p, self.seed, stream))
-        self._kept = (x.shape, stream)
+        self._kept = (x.shape, x.engine, stream)
         return out
 
     def forward(self, input):
@@ -258,8 +258,8 @@ class Dropout(Module):
     def backward(self, gradient):
         if self._kept is None:
             raise _ffi.StateError(_ffi.RST_ERR_STATE, "Dropout.backward without a forward")
-        g = as_array2(gradient)
-        shape, stream = self._kept
+        shape, engine, stream = self._kept
+        g = as_array2(gradient, engine)
         if g.shape != shape:
             raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "gradient %r vs input %r" % (g.shape, shape))
         self._kept = None
@@ -689,6 +689,17 @@ class Sequential(Module):
         self._drop_plan()
         return self.layers.pop(index)
 
+    def _engine(self):
+        """The engine of the first layer that has one; None: no layer is bound to any."""
+        for layer in self.layers:
+            if isinstance(layer, (Linear, LayerNorm)):
+                return layer.engine
+            inner = layer.inner if isinstance(layer, Residual) else layer
+            engine = inner._engine() if isinstance(inner, Sequential) else None
+            if engine is not None:
+                return engine
+        return None
+
     def _output_size(self, width):
         """Columns of what the layers return for an input of ``width`` columns; None where a layer of the caller's own
         decides that."""
@@ -725,6 +736,8 @@ class Sequential(Module):
         """Layer by layer; residual (or None) is added to the result, by the last layer where it can."""
         x = input
         last = self._prev_real(len(self.layers))  # (-1: nothing but Identity)
+        if last >= 0 and type(self.layers[self._next_real(-1)]) in _ANY_ENGINE:
+            x = as_array2(input, self._engine())  # (the layer alone would put a host array on the default engine)
         skip = set()
         for i, layer in enumerate(self.layers):
             if i in skip:
@@ -825,30 +838,31 @@ class Residual(Module):
             self.inner = inner
         else:
             self.inner = Sequential(list(inner) if isinstance(inner, (list, tuple)) else [inner])
-        self._shape = None
+        self._kept = None  # (shape, engine) of the last forward's input
 
     @classmethod
     def new(cls, inner):
         return cls(inner)
 
     def forward(self, input):
-        x = as_array2(input)
+        x = as_array2(input, self.inner._engine())
         self.inner._drop_plan()  # (a compiled form would add in a pass of its own)
         wide = self.inner._output_size(x.cols)
         if wide is not None and wide != x.cols:
             raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "a residual of %d features around layers that return %d"
                                   % (x.cols, wide))
         out = self.inner._layers_forward(x, x)
-        self._shape = x.shape
+        self._kept = (x.shape, x.engine)
         return out
 
     def backward(self, gradient):
-        if self._shape is None:
+        if self._kept is None:
             raise _ffi.StateError(_ffi.RST_ERR_STATE, "Residual.backward without a forward")
-        g = as_array2(gradient)
-        if g.shape != self._shape:
-            raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "gradient %r vs input %r" % (g.shape, self._shape))
-        self._shape = None
+        shape, engine = self._kept
+        g = as_array2(gradient, engine)
+        if g.shape != shape:
+            raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "gradient %r vs input %r" % (g.shape, shape))
+        self._kept = None
         return self.inner._layers_backward(g, g)
 
     def parameters(self):
@@ -864,6 +878,8 @@ class Residual(Module):
         return "Residual(%s)" % ", ".join(repr(l) for l in self.inner.layers)
 
 
+# layers that take an array of any engine
+_ANY_ENGINE = (ReLU, Softmax, GELU, SiLU, Dropout)
 # layers that return as many columns as they are given
 _SAME_WIDTH = (Identity, ReLU, Softmax, GELU, SiLU, Dropout, LayerNorm, Residual)
 

@@ -5,6 +5,7 @@ import os
 import shutil
 import subprocess
 
+import numpy as np
 import pytest
 
 import rstorch_amd as rs
@@ -173,6 +174,27 @@ def test_a_residual_around_layers_that_change_the_width(recorder):
         with pytest.raises(rs.ShapeError):
             rs.Residual(inner).forward(recorder.empty(4, 6))
         assert not recorder.taken() or isinstance(inner[1], Resize)
+
+
+@pytest.mark.parametrize("first", [rs.GELU, rs.SiLU, rs.ReLU, rs.Dropout, rs.Identity])
+@pytest.mark.parametrize("outer", [rs.Sequential, rs.Residual])
+def test_host_arrays_go_to_the_engine_of_the_layers(recorder, monkeypatch, first, outer):
+    """Layers on an engine of their own (another stream, possibly another GPU): nothing of theirs runs on the default one."""
+    other = Recorder()
+    monkeypatch.setattr("rstorch_amd.engine.default_engine", lambda: other)
+    monkeypatch.setattr("rstorch_amd.module.default_engine", lambda: other)
+    monkeypatch.setattr(rs.Sequential, "compile_enabled", False)  # (a compiled list keeps to its layers' engine anyway)
+    lin = lambda: rs.Linear(6, 6, engine=recorder)
+    x = np.zeros((4, 6))
+    for inner in ([first(), lin()], [first(), rs.LayerNorm(6, engine=recorder), first()], [lin(), first()],
+                  [first(), rs.Sequential([lin()])], [first(), rs.Residual([first(), lin()])]):
+        model = outer(inner)
+        out = model.forward(x)
+        assert out.engine is recorder
+        assert rs.as_array2(model.backward(x)).engine is recorder
+    assert not other.taken()
+    # layers that are bound to no engine keep using the default one
+    assert outer([rs.GELU(), rs.Dropout(0.5)]).forward(x).engine is other
 
 
 @pytest.mark.skipif(shutil.which("hipcc") is None and not os.path.exists("/opt/rocm/bin/hipcc"),
