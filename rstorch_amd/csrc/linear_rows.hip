@@ -37,19 +37,19 @@ __device__ __forceinline__ double activate(int activation, double z) {
 }
 
 // ROWS: rows of x, rounded up to a power of two (rows beyond the real ones repeat the last and are not
-// stored); WAVES wavefronts per workgroup; DEPTH steps of 128 values in flight.
+// stored); WAVES wavefronts per workgroup; DEPTH steps of 128 values in flight; `begin_feature`: the launch's first.
 template <int ROWS, int WAVES, int DEPTH>
 __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(const double* __restrict__ x,
                                                                  const double* __restrict__ w,
                                                                  const double* __restrict__ bias, double* out,
                                                                  const ActEpilogue e, int rows, size_t features,
-                                                                 size_t length) {
+                                                                 size_t length, size_t begin_feature) {
   constexpr int VALUES = ROWS * kFeatures;
   constexpr int LOG = VALUES == 4 ? 2 : VALUES == 8 ? 3 : VALUES == 16 ? 4 : 5;
   static_assert(VALUES == 1 << LOG, "four to thirty-two sums");
   __shared__ double part[WAVES][VALUES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const size_t first = (size_t)blockIdx.x * kFeatures;
+  const size_t first = begin_feature + (size_t)blockIdx.x * kFeatures;
   const double* wr[kFeatures];
   const double* xr[ROWS];
 #pragma unroll
@@ -130,18 +130,28 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(const double* _
   }
 }
 
+template <int ROWS, int DEPTH, int WAVES>
+int launch_waves(hipStream_t s, const double* x, const double* w, const double* bias, double* out, const ActEpilogue& e,
+                 int rows, size_t features, size_t length) {
+  // a grid has fewer than 2^32 threads; more features take several launches, each of them long
+  constexpr size_t kMostGroups = ((size_t)1 << 31) / (64 * WAVES);
+  const size_t groups = (features + kFeatures - 1) / kFeatures;
+  for (size_t g = 0; g < groups; g += kMostGroups) {
+    const dim3 grid((unsigned)(groups - g < kMostGroups ? groups - g : kMostGroups));
+    hipLaunchKernelGGL((linear_rows_kernel<ROWS, WAVES, DEPTH>), grid, dim3(64 * WAVES), 0, s, x, w, bias, out, e, rows,
+                       features, length, g * kFeatures);
+    RST_HIP(hipGetLastError());
+  }
+  return RST_OK;
+}
+
 template <int ROWS, int DEPTH>
-void launch(hipStream_t s, const double* x, const double* w, const double* bias, double* out, const ActEpilogue& e,
-            int rows, size_t features, size_t length) {
-  const dim3 grid((unsigned)((features + kFeatures - 1) / kFeatures));
+int launch(hipStream_t s, const double* x, const double* w, const double* bias, double* out, const ActEpilogue& e,
+           int rows, size_t features, size_t length) {
   // few weight rows: more wavefronts on each, so that the chip has loads enough in flight
   constexpr int MANY = ROWS == 8 ? 8 : 16;  // (sixteen leave 128 registers, and eight rows need more)
-  if (features <= 1024)
-    hipLaunchKernelGGL((linear_rows_kernel<ROWS, MANY, DEPTH>), grid, dim3(64 * MANY), 0, s, x, w, bias, out, e, rows,
-                       features, length);
-  else
-    hipLaunchKernelGGL((linear_rows_kernel<ROWS, 4, DEPTH>), grid, dim3(256), 0, s, x, w, bias, out, e, rows, features,
-                       length);
+  if (features <= 1024) return launch_waves<ROWS, DEPTH, MANY>(s, x, w, bias, out, e, rows, features, length);
+  return launch_waves<ROWS, DEPTH, 4>(s, x, w, bias, out, e, rows, features, length);
 }
 
 }  // namespace
@@ -153,12 +163,10 @@ bool linear_rows_supported(size_t rows, size_t features, size_t length) {
 
 int launch_linear_rows(hipStream_t s, const double* x, const double* w, const double* bias, double* out,
                        const ActEpilogue& e, size_t rows, size_t features, size_t length) {
-  if (rows == 1) launch<1, 4>(s, x, w, bias, out, e, (int)rows, features, length);
-  else if (rows == 2) launch<2, 4>(s, x, w, bias, out, e, (int)rows, features, length);
-  else if (rows <= 4) launch<4, 2>(s, x, w, bias, out, e, (int)rows, features, length);
-  else launch<8, 1>(s, x, w, bias, out, e, (int)rows, features, length);
-  RST_HIP(hipGetLastError());
-  return RST_OK;
+  if (rows == 1) return launch<1, 4>(s, x, w, bias, out, e, (int)rows, features, length);
+  if (rows == 2) return launch<2, 4>(s, x, w, bias, out, e, (int)rows, features, length);
+  if (rows <= 4) return launch<4, 2>(s, x, w, bias, out, e, (int)rows, features, length);
+  return launch<8, 1>(s, x, w, bias, out, e, (int)rows, features, length);
 }
 
 }  // namespace rst
