@@ -125,7 +125,9 @@ int rst_softmax_backward(rst_engine* engine, const double* grad, const double* o
  *      backward pass).  Parameter gradients are divided by the number of rows, as Linear's are
  *      (src/module/linear.rs:62-66), and overwritten, never accumulated.  Arrays need their 8-byte
  *      alignment only and have any extents up to 2^31 - 128 (layer norm's backward pass over rows of one value:
- *      2^23 rows; more is RST_ERR_UNSUPPORTED).  Nothing here allocates or waits; launches recorded into
+ *      2^23 rows; the outputs of a product: fewer than 2^23 tiles of 128 x 128, as 2^30 - 128 rows of up to 128
+ *      columns are, but for a forward pass of up to eight rows; more is RST_ERR_UNSUPPORTED, and nothing is
+ *      launched).  Nothing here allocates or waits; launches recorded into
  *      a graph of the caller's use the engine's scratch as the eager ones do: graphs of one engine run
  *      one at a time, on its stream ------------------------------------------------------------------ */
 /* RST_ACT_GELU: z (1 + erf(z / sqrt 2)) / 2;  RST_ACT_GELU_TANH: z (1 + tanh(sqrt(2 / pi) (z +

@@ -142,6 +142,8 @@ int rst_linear_act_backward(rst_engine* e, const double* grad, const double* pre
   RST_TRY(check_dim("linear_act_backward", batch, "batch"));
   RST_TRY(check_dim("linear_act_backward", in_features, "in_features"));
   RST_TRY(check_dim("linear_act_backward", out_features, "out_features"));
+  RST_TRY(check_contraction(out_features, in_features));
+  if (grad_input) RST_TRY(check_contraction(batch, in_features));
   if (activation != RST_ACT_NONE) {
     RST_TRY(launch_act_backward(e->stream, activation, grad, pre, nullptr, grad_pre, batch * out_features));
     grad = grad_pre;

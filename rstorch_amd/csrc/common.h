@@ -83,6 +83,9 @@ struct ActEpilogue {
 };
 
 int launch_gemm(hipStream_t stream, const GemmDesc& d);
+// RST_ERR_UNSUPPORTED where launch_gemm would refuse a rows x cols result (2^23 tiles of 128x128 and more): what an
+// entry point of several launches asks before the first of them
+int check_contraction(size_t rows, size_t cols);
 // Two independent contractions, the input gradient of one layer (A contraction-contiguous, B
 // output-contiguous) and the weight gradient of another (both output-contiguous), in one grid.
 // Possible when both run as unsplit 128x128 direct-to-LDS tiles and the first alone would

@@ -1370,6 +1370,13 @@ int compute_units() {
   return cus;
 }
 
+// a grid has fewer than 2^32 threads
+bool grid_fits(long long blocks, int threads) { return blocks * threads <= 0xffffffffLL; }
+int check_grid(long long blocks, int threads) {
+  if (!grid_fits(blocks, threads)) return fail(RST_ERR_UNSUPPORTED, "a contraction of %lld workgroups", blocks);
+  return RST_OK;
+}
+
 // want_split > 1: cut K into that many slices (the caller has checked the workspace)
 template <bool A_KC, bool B_KC>
 int launch_dma(hipStream_t stream, GemmParams p, int want_split = 0, const ActEpilogue* e = nullptr) {
@@ -1397,7 +1404,7 @@ int launch_dma(hipStream_t stream, GemmParams p, int want_split = 0, const ActEp
     p.ws_colsum = p.ws + (size_t)2 * p.M * p.N;
     blocks *= 2;
   }
-  if (blocks > 0x7fffffffLL) return fail(RST_ERR_UNSUPPORTED, "contraction grid too large");
+  RST_TRY(check_grid(blocks, 512));
   // more than one round of workgroups (two per CU fit): stagger the first round by 0.4 us per K step
   p.first_round = 2 * compute_units();
   p.dephase_ticks = blocks > p.first_round ? (p.steps_per_split < 250 ? 40 * p.steps_per_split : 10000) : 0;
@@ -1433,7 +1440,7 @@ int launch_dma64(hipStream_t stream, GemmParams p, int slices, const ActEpilogue
       blocks *= p.split_k;
     }
   }
-  if (blocks > 0x7fffffffLL) return fail(RST_ERR_UNSUPPORTED, "contraction grid too large");
+  RST_TRY(check_grid(blocks, 256));
   RST_OBSERVE_GEMM(GemmKernel::kDma64, 64, 64, 2, 2, true, B_KC, p.unaligned == 0, 0, blocks, 256, &p, nullptr, 0, nullptr, e != nullptr);
   if (e) {
     hipLaunchKernelGGL(gemm_f64_mfma_dma64_act<B_KC>, dim3((unsigned)blocks), dim3(256), 0, stream, p, *e);
@@ -1538,7 +1545,7 @@ int launch_one(hipStream_t stream, GemmParams p, long long split_below = 256, lo
   if (e && BM == 32) plan_act_slices(&self, 1);
   else plan_slices(p, blocks, split_below, want_blocks);
   blocks *= p.split_k;
-  if (blocks > 0x7fffffffLL) return fail(RST_ERR_UNSUPPORTED, "contraction grid too large");
+  RST_TRY(check_grid(blocks, WGM * WGN * 64));
   const bool burst = BM == 32 && BN == 32 && blocks <= compute_units();
   RST_OBSERVE_GEMM(GemmKernel::kStaged, BM, BN, WGM, WGN, A_KC, B_KC, VEC, burst ? kBurst : 0, blocks, WGM * WGN * 64, &p, nullptr, 0, nullptr, e != nullptr);
   if constexpr (A_KC) {
@@ -1830,6 +1837,11 @@ bool takes_plain_dma(const GemmDesc& d, long long* blocks) {
 
 }  // namespace
 
+// (from 256 tiles of 128x128 on every route takes those, with 512 threads each, and below that no grid is near the limit)
+int check_contraction(size_t rows, size_t cols) {
+  return check_grid((long long)((rows + 127) / 128) * (long long)((cols + 127) / 128), 512);
+}
+
 int launch_gemm(hipStream_t stream, const GemmDesc& d) {
   if (d.M <= 0 || d.N <= 0) return RST_OK;
   const GemmParams p = make_params(d);
@@ -2064,7 +2076,8 @@ int launch_gemm_group(hipStream_t stream, const GemmDesc* d, int count) {
     }
     g.p[i] = p;
   }
-  if (blocks > 0x7fffffffLL || reduce_blocks > 0x7fffffffLL) return fail(RST_ERR_UNSUPPORTED, "contraction grid too large");
+  RST_TRY(check_grid(blocks, 256));
+  RST_TRY(check_grid(reduce_blocks, 256));
   g.first_block[count] = (int)blocks;
   g.first_reduce_block[count] = (int)reduce_blocks;
   const bool burst = blocks <= compute_units();
@@ -2156,7 +2169,7 @@ int launch_grads_act(hipStream_t stream, const GemmDesc& weight_grad, const Gemm
     reduce_blocks += (long long)(((size_t)p.M * p.N + 255) / 256);
   }
   if (ws_used > g.p[0].ws_capacity) return fail(RST_ERR_INVALID_ARGUMENT, "group workspace exhausted");
-  if (blocks > 0x7fffffffLL || reduce_blocks > 0x7fffffffLL) return fail(RST_ERR_UNSUPPORTED, "contraction grid too large");
+  if (!grid_fits(blocks, 256) || !grid_fits(reduce_blocks, 256)) return RST_OK;  // (apart they take larger tiles)
   *taken = true;
   const bool burst = blocks <= compute_units();
 #ifdef RST_GEMM_LAUNCH_OBSERVER
@@ -2179,7 +2192,7 @@ bool can_pair_gemm(const GemmDesc& input_grad, const GemmDesc& weight_grad) {
   const bool layouts = input_grad.a_kc && !input_grad.b_kc && !weight_grad.a_kc && !weight_grad.b_kc && !input_grad.act;
   // worth it when the input gradient alone would leave one workgroup per CU
   return layouts && takes_plain_dma(input_grad, &b1) && takes_plain_dma(weight_grad, &b2) && b1 < 512 &&
-         b1 % 8 == 0 && b2 >= b1 && b1 + b2 <= 0x7fffffffLL;
+         b1 % 8 == 0 && b2 >= b1 && grid_fits(b1 + b2, 512);
 }
 
 int launch_gemm_pair(hipStream_t stream, const GemmDesc& input_grad, const GemmDesc& weight_grad) {
@@ -2201,7 +2214,7 @@ bool can_pair_grads_act(const GemmDesc& weight_grad, const GemmDesc& input_grad)
   if (!input_grad.act || !input_grad.a_kc || input_grad.b_kc || weight_grad.a_kc || weight_grad.b_kc) return false;
   if (!takes_plain_dma(weight_grad, &b1) || !takes_plain_dma(input_grad, &b2)) return false;
   if (b1 > b2) std::swap(b1, b2);
-  return b1 < 512 && b1 % 8 == 0 && b1 + b2 <= 0x7fffffffLL;
+  return b1 < 512 && b1 % 8 == 0 && grid_fits(b1 + b2, 512);
 }
 
 int launch_gemm_grads_act(hipStream_t stream, const GemmDesc& weight_grad, const GemmDesc& input_grad) {

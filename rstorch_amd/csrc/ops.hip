@@ -182,6 +182,8 @@ int rst_linear_backward(rst_engine* e, const double* grad, const double* x, cons
   RST_TRY(check_dim(batch, "batch"));
   RST_TRY(check_dim(in_features, "in_features"));
   RST_TRY(check_dim(out_features, "out_features"));
+  RST_TRY(check_contraction(out_features, in_features));
+  if (grad_input) RST_TRY(check_contraction(batch, in_features));
   return engine_linear_backward(e, grad, x, weight, grad_weight, grad_bias, grad_input, relu_mask_source, nullptr,
                                 batch, in_features, out_features);
 }
