@@ -1370,6 +1370,9 @@ int compute_units() {
   return cus;
 }
 
+// pieces of `tile` that cover `extent` (which is up to 2^31 - 1: the sum of the two is no int)
+int tile_count(int extent, int tile) { return (int)(((long long)extent + tile - 1) / tile); }
+
 // a grid has fewer than 2^32 threads
 bool grid_fits(long long blocks, int threads) { return blocks * threads <= 0xffffffffLL; }
 int check_grid(long long blocks, int threads) {
@@ -1380,8 +1383,8 @@ int check_grid(long long blocks, int threads) {
 // want_split > 1: cut K into that many slices (the caller has checked the workspace)
 template <bool A_KC, bool B_KC>
 int launch_dma(hipStream_t stream, GemmParams p, int want_split = 0, const ActEpilogue* e = nullptr) {
-  p.tiles_m = (p.M + 127) / 128;
-  p.tiles_n = (p.N + 127) / 128;
+  p.tiles_m = tile_count(p.M, 128);
+  p.tiles_n = tile_count(p.N, 128);
   p.split_k = 1;
   p.steps_per_split = dma_whole_steps(p.K, p.k_reserve);
   long long blocks = (long long)p.tiles_m * p.tiles_n;
@@ -1426,8 +1429,8 @@ int launch_dma(hipStream_t stream, GemmParams p, int want_split = 0, const ActEp
 // 64x64 direct-to-LDS tiles, optionally on `slices` K slices (the caller has checked the workspace)
 template <bool B_KC>
 int launch_dma64(hipStream_t stream, GemmParams p, int slices, const ActEpilogue* e = nullptr) {
-  p.tiles_m = (p.M + kT64 - 1) / kT64;
-  p.tiles_n = (p.N + kT64 - 1) / kT64;
+  p.tiles_m = tile_count(p.M, kT64);
+  p.tiles_n = tile_count(p.N, kT64);
   const int nk = dma_whole_steps(p.K, p.k_reserve);
   p.split_k = 1;
   p.steps_per_split = nk;
@@ -1456,7 +1459,7 @@ int launch_dma64(hipStream_t stream, GemmParams p, int slices, const ActEpilogue
 // Few output tiles (`blocks` < split_below) but a long contraction: the number of K slices that
 // fills the chip (want_blocks workgroups, about eight per CU), 1 = none.
 long long small_tile_slices(const GemmParams& p, long long blocks, long long split_below, long long want_blocks) {
-  const int nk = (p.K + BK - 1) / BK;
+  const int nk = tile_count(p.K, BK);
   if (!(blocks < split_below && nk >= 8 && p.ws != nullptr)) return 1;
   long long want = (want_blocks + blocks - 1) / blocks;
   if (want > 64) want = 64;                                // keep the ordered reduction short
@@ -1475,7 +1478,7 @@ constexpr long long kSmallTileSplitBelow = 512;
 
 // Fills in split_k, steps_per_split and ws_colsum of a small-tile launch of `blocks` output tiles.
 void plan_slices(GemmParams& p, long long blocks, long long split_below, long long want_blocks) {
-  const int nk = (p.K + BK - 1) / BK;
+  const int nk = tile_count(p.K, BK);
   p.split_k = 1;
   p.steps_per_split = nk;
   const long long s = small_tile_slices(p, blocks, split_below, want_blocks);
@@ -1499,8 +1502,8 @@ double plan_act_slices(GemmParams* const* p, int count) {
   long long tiles[2] = {0, 0};
   size_t room = p[0]->ws != nullptr ? p[0]->ws_capacity : 0;
   for (int i = 0; i < count; ++i) {
-    nk[i] = (p[i]->K + BK - 1) / BK;
-    tiles[i] = (long long)((p[i]->M + 31) / 32) * ((p[i]->N + 31) / 32);
+    nk[i] = tile_count(p[i]->K, BK);
+    tiles[i] = (long long)tile_count(p[i]->M, 32) * tile_count(p[i]->N, 32);
     if (nk[i] > longest) longest = nk[i];
   }
   const double join = count > 1 ? 3.7 : 2.6;
@@ -1538,8 +1541,8 @@ double plan_act_slices(GemmParams* const* p, int count) {
 template <int BM, int BN, int WGM, int WGN, bool A_KC, bool B_KC, bool VEC>
 int launch_one(hipStream_t stream, GemmParams p, long long split_below = 256, long long want_blocks = 2048,
                const ActEpilogue* e = nullptr) {
-  p.tiles_m = (p.M + BM - 1) / BM;
-  p.tiles_n = (p.N + BN - 1) / BN;
+  p.tiles_m = tile_count(p.M, BM);
+  p.tiles_n = tile_count(p.N, BN);
   long long blocks = (long long)p.tiles_m * p.tiles_n;
   GemmParams* const self = &p;
   if (e && BM == 32) plan_act_slices(&self, 1);
@@ -1620,7 +1623,7 @@ int band_slices(const GemmParams& p, long long t128) {
 
 Route choose_route(const GemmParams& p, int* dma_slices, bool is_a_kc = false, bool is_b_kc = false) {
   auto tiles = [&](int bm, int bn) {
-    return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn);
+    return (long long)tile_count(p.M, bm) * tile_count(p.N, bn);
   };
   // (leading dimensions below 2^22 doubles keep the 32-bit lane offsets of the tile DMA in range;
   // the tile DMA needs no more than the 8-byte alignment every operand has)
@@ -1732,7 +1735,7 @@ struct ActPlan {
 double dma_cost(const GemmParams& p, int tile, int slices) {
   const double one = tile == 128 ? 1.84 : 0.535, two = tile == 128 ? 3.65 : 1.0;
   const int nk = dma_whole_steps(p.K, p.k_reserve), steps = (nk + slices - 1) / slices;
-  const long long groups = (long long)((p.M + tile - 1) / tile) * ((p.N + tile - 1) / tile) * slices, rem = groups % 512;
+  const long long groups = (long long)tile_count(p.M, tile) * tile_count(p.N, tile) * slices, rem = groups % 512;
   double c = 6.0 + (double)(groups / 512) * two * steps + (rem > 256 ? two * steps : rem > 0 ? one * steps : 0.0);
   if (slices > 1) c += 16.0 * slices * (double)p.M * (double)p.N / 5.2e6;
   return c;
@@ -1757,7 +1760,7 @@ ActPlan plan_act(const GemmParams& p, bool a_kc, bool b_kc) {
   };
   consider(128, 8);
   // (from 512 tiles on the larger ones have the chip full, and the smaller would read every operand twice as often)
-  if (a_kc && (long long)((p.M + 127) / 128) * ((p.N + 127) / 128) < 512) consider(64, 16);
+  if (a_kc && (long long)tile_count(p.M, 128) * tile_count(p.N, 128) < 512) consider(64, 16);
   return best;
 }
 
@@ -1829,7 +1832,7 @@ GemmParams make_params(const GemmDesc& d) {
 bool takes_plain_dma(const GemmDesc& d, long long* blocks) {
   if (d.M < 2 || d.N < 2 || d.K <= 0) return false;
   if (d.lda >= (1L << 22) || d.ldb >= (1L << 22)) return false;
-  *blocks = (long long)((d.M + 127) / 128) * ((d.N + 127) / 128);
+  *blocks = (long long)tile_count(d.M, 128) * tile_count(d.N, 128);
   if (*blocks < 256) return false;
   const GemmParams p = make_params(d);
   return !(*blocks < 512 && dma_whole_steps(p.K, p.k_reserve) >= kSplitMinSteps && d.workspace != nullptr);
@@ -1860,8 +1863,8 @@ int max_gemm_group() { return kMaxGroup; }
 namespace {
 // the slices of a group member: what launch_gemm would choose for it alone
 void plan_group_member(GemmParams& p) {
-  p.tiles_m = (p.M + 31) / 32;
-  p.tiles_n = (p.N + 31) / 32;
+  p.tiles_m = tile_count(p.M, 32);
+  p.tiles_n = tile_count(p.N, 32);
   plan_slices(p, (long long)p.tiles_m * p.tiles_n, kSmallTileSplitBelow, 2048);
 }
 }  // namespace
@@ -1898,7 +1901,7 @@ constexpr int kDmaGroupGrid = 256;
 // the shared workspace)
 bool dma_group_member(const GemmDesc& d) {
   return !d.a_kc && !d.b_kc && d.K / BK >= 2 * kDmaGroupMinSteps && d.M >= 2 && d.N >= 2 &&
-         (long long)((d.M + 127) / 128) * ((d.N + 127) / 128) <= 8 && d.lda < (1L << 22) && d.ldb < (1L << 22) &&
+         (long long)tile_count(d.M, 128) * tile_count(d.N, 128) <= 8 && d.lda < (1L << 22) && d.ldb < (1L << 22) &&
          d.workspace != nullptr;
 }
 
@@ -1933,7 +1936,7 @@ bool plan_dma_group(const GemmDesc* d, int count, GemmGroup* g, long long* block
   double outputs = 0.0;
   for (int i = 0; i < count; ++i) {
     if (!dma_group_member(d[i])) return false;
-    tiles += (long long)((d[i].M + 127) / 128) * ((d[i].N + 127) / 128);
+    tiles += (long long)tile_count(d[i].M, 128) * tile_count(d[i].N, 128);
     outputs += (double)d[i].M * d[i].N;
   }
   if (tiles > kDmaGroupGrid / 8) return false;
@@ -1975,7 +1978,7 @@ bool plan_dma_group(const GemmDesc* d, int count, GemmGroup* g, long long* block
     // six MFMAs per SIMD take (measured: 0.8 us against 2.2 us for a full tile's sixteen)
     if (cost[i] < 6) cost[i] = 6;
     if (cost[i] > cost_max) cost_max = cost[i];
-    weight += (double)cost[i] * (double)(((piece[i].M + 127) / 128) * ((piece[i].N + 127) / 128));
+    weight += (double)cost[i] * (double)(tile_count(piece[i].M, 128) * tile_count(piece[i].N, 128));
   }
   const double full_slices = (double)kDmaGroupGrid * (double)cost_max / weight;  // of a piece of the highest cost
   long long blocks = 0, reduce_blocks = 0;
@@ -1983,8 +1986,8 @@ bool plan_dma_group(const GemmDesc* d, int count, GemmGroup* g, long long* block
   g->count = pieces;
   for (int i = 0; i < pieces; ++i) {
     GemmParams p = make_params(piece[i]);
-    p.tiles_m = (p.M + 127) / 128;
-    p.tiles_n = (p.N + 127) / 128;
+    p.tiles_m = tile_count(p.M, 128);
+    p.tiles_n = tile_count(p.N, 128);
     const int nk = dma_whole_steps(p.K, p.k_reserve);
     long long s = (long long)(full_slices * (double)cost[i] / (double)cost_max + 0.5);
     if (s > kDmaGroupMaxSlices) s = kDmaGroupMaxSlices;
@@ -2154,8 +2157,8 @@ int launch_grads_act(hipStream_t stream, const GemmDesc& weight_grad, const Gemm
   size_t ws_used = 0;
   for (int i = 0; i < 2; ++i) {
     GemmParams& p = g.p[i];
-    p.tiles_m = (p.M + 31) / 32;
-    p.tiles_n = (p.N + 31) / 32;
+    p.tiles_m = tile_count(p.M, 32);
+    p.tiles_n = tile_count(p.N, 32);
     if (i == 1) {
       g.first_block = (int)blocks;
       g.first_reduce_block = (int)reduce_blocks;
@@ -2199,8 +2202,8 @@ int launch_gemm_pair(hipStream_t stream, const GemmDesc& input_grad, const GemmD
   if (!can_pair_gemm(input_grad, weight_grad))
     return fail(RST_ERR_INVALID_ARGUMENT, "these two contractions cannot share a grid");
   GemmParams p1 = make_params(input_grad), p2 = make_params(weight_grad);
-  p1.tiles_m = (p1.M + 127) / 128; p1.tiles_n = (p1.N + 127) / 128; p1.steps_per_split = dma_whole_steps(p1.K, p1.k_reserve);
-  p2.tiles_m = (p2.M + 127) / 128; p2.tiles_n = (p2.N + 127) / 128; p2.steps_per_split = dma_whole_steps(p2.K, p2.k_reserve);
+  p1.tiles_m = tile_count(p1.M, 128); p1.tiles_n = tile_count(p1.N, 128); p1.steps_per_split = dma_whole_steps(p1.K, p1.k_reserve);
+  p2.tiles_m = tile_count(p2.M, 128); p2.tiles_n = tile_count(p2.N, 128); p2.steps_per_split = dma_whole_steps(p2.K, p2.k_reserve);
   const long long b1 = (long long)p1.tiles_m * p1.tiles_n, b2 = (long long)p2.tiles_m * p2.tiles_n;
   RST_OBSERVE_GEMM(GemmKernel::kDma128Pair, 128, 128, 2, 4, true, false, true, 0, b1 + b2, 512, &p1, &p2, (int)b1, nullptr);
   hipLaunchKernelGGL((gemm_f64_mfma_dma_pair<true, false, false, false>), dim3((unsigned)(b1 + b2)), dim3(512),
@@ -2222,8 +2225,8 @@ int launch_gemm_grads_act(hipStream_t stream, const GemmDesc& weight_grad, const
     return fail(RST_ERR_INVALID_ARGUMENT, "these two contractions cannot share a grid");
   GemmParams dw = make_params(weight_grad), dx = make_params(input_grad);
   for (GemmParams* p : {&dw, &dx}) {
-    p->tiles_m = (p->M + 127) / 128;
-    p->tiles_n = (p->N + 127) / 128;
+    p->tiles_m = tile_count(p->M, 128);
+    p->tiles_n = tile_count(p->N, 128);
     p->steps_per_split = dma_whole_steps(p->K, p->k_reserve);
   }
   const long long bw = (long long)dw.tiles_m * dw.tiles_n, bx = (long long)dx.tiles_m * dx.tiles_n;

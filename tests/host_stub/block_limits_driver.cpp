@@ -100,6 +100,22 @@ int main() {
   // (the weight gradient alone is small whatever the batch)
   LAUNCHES(backward(last + 1, 3, 2, false, RST_ACT_NONE), 2);
   LAUNCHES(plain_backward(last + 1, 3, 2, false), 2);
+  // the largest extents: refused or run, without an overflow on the way
+  for (size_t batch : {9u, 100u, 129u, 5000u}) {
+    REFUSED(linear(batch, 1, most));
+    REFUSED(linear(most, 1, batch));
+    REFUSED(backward(most, batch, 1));
+    REFUSED(backward(1, most, batch));
+    REFUSED(backward(1, batch, most));
+    LAUNCHES(linear(batch, most, 1), 2);
+    for (size_t extent : {(size_t)INT_MAX - 1, (size_t)INT_MAX}) {
+      REFUSED(rst_linear_forward(e, at(0), at(1), at(2), at(5), batch, 1, extent, 0));
+      REFUSED(rst_linear_forward(e, at(0), at(1), at(2), at(5), extent, 1, batch, 0));
+      REFUSED(plain_backward(extent, batch, 1));
+      REFUSED(plain_backward(1, batch, extent));
+    }
+  }
+  REFUSED(linear(most, most, most));
   if (rst_engine_destroy(e) != RST_OK) return 1;
   std::printf("block limits ok\n");
   return 0;
