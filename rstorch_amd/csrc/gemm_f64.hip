@@ -2120,6 +2120,7 @@ double grads_apart(const GemmParams* p) {
   return sum;
 }
 
+#ifdef RST_GEMM_LAUNCH_OBSERVER
 // (for the launch observer)
 GemmGroup group_of(const GradsPair& g, int blocks, int reduce_blocks) {
   GemmGroup all{};
@@ -2133,6 +2134,7 @@ GemmGroup group_of(const GradsPair& g, int blocks, int reduce_blocks) {
   all.p[1] = g.p[1];
   return all;
 }
+#endif
 }  // namespace
 
 // Both gradients of a layer in one grid of 32x32 tiles, or each on the tiles that suit it: whichever the two models
@@ -2151,8 +2153,10 @@ int launch_grads_act(hipStream_t stream, const GemmDesc& weight_grad, const Gemm
   g.p[1] = make_params(input_grad);
   GemmParams* const both[2] = {&g.p[0], &g.p[1]};
   const double together = plan_act_slices(both, 2);
-  // (none of the 46 below 1 GFLOP was faster apart)
-  if (4.0 * weight_grad.M * weight_grad.N * (double)weight_grad.K >= 1e8 && together >= grads_apart(g.p)) return RST_OK;
+  // (below 1 GFLOP the model of the separate launches is too short where one product is a thin 32x32 one and the other has
+  // hundreds of larger tiles: 32 layers of 0.1 to 1 GFLOP, seventeen of which it would keep apart, took 0.46 to 0.96 times as
+  // long together - 7 rows of 4361 -> 4431 115 us and 182, 2186 of 1794 -> 62 49 and 57 - but for one at 1.01)
+  if (4.0 * weight_grad.M * weight_grad.N * (double)weight_grad.K >= 1e9 && together >= grads_apart(g.p)) return RST_OK;
   long long blocks = 0, reduce_blocks = 0;
   size_t ws_used = 0;
   for (int i = 0; i < 2; ++i) {

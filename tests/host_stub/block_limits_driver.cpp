@@ -10,7 +10,8 @@
 #include "../../rstorch_amd/csrc/common.h"
 #include "../../rstorch_amd/csrc/gemm_addressing.h"
 
-void rst::observe_gemm_launch(const rst::GemmLaunch&) {}
+static long g_shared = 0;  // grids of 32x32 tiles that both gradients of a layer share
+void rst::observe_gemm_launch(const rst::GemmLaunch& l) { g_shared += l.kernel == rst::GemmKernel::kStagedMixedGroup; }
 
 extern "C" long hip_stub_launch_count();
 
@@ -116,6 +117,16 @@ int main() {
     }
   }
   REFUSED(linear(most, most, most));
+  // below 1 GFLOP both gradients share a grid, whatever the shape
+  const size_t thin[][3] = {{7, 4361, 4431}, {21, 3858, 2909}, {2186, 1794, 62}, {13786, 282, 35}, {3466, 2176, 7}, {22, 1999, 3212},
+                            {49, 1225, 3940}, {11550, 1720, 6}, {15896, 482, 29}, {1, 1, 1}, {32, 784, 100}};
+  for (auto& d : thin) {
+    g_shared = 0;
+    if (backward(d[0], d[1], d[2]) != RST_OK || g_shared != 1) {
+      std::fprintf(stderr, "%zu rows of %zu -> %zu: %ld shared grids\n", d[0], d[1], d[2], g_shared);
+      return 1;
+    }
+  }
   if (rst_engine_destroy(e) != RST_OK) return 1;
   std::printf("block limits ok\n");
   return 0;
