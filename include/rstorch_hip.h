@@ -127,9 +127,10 @@ int rst_softmax_backward(rst_engine* engine, const double* grad, const double* o
  *      alignment only and have any extents up to 2^31 - 128 (layer norm's backward pass over rows of one value:
  *      2^23 rows; the outputs of a product: fewer than 2^23 tiles of 128 x 128, as 2^30 - 128 rows of up to 128
  *      columns are, but for a forward pass of up to eight rows; more is RST_ERR_UNSUPPORTED, and nothing is
- *      launched).  Nothing here allocates or waits; launches recorded into
- *      a graph of the caller's use the engine's scratch as the eager ones do: graphs of one engine run
- *      one at a time, on its stream ------------------------------------------------------------------ */
+ *      launched).  Where a call does not say that an output may be an operand, the output shares no element
+ *      with another array of the call (rst_linear_act_* check that, the others do not).  Nothing here allocates
+ *      or waits; launches recorded into a graph of the caller's use the engine's scratch as the eager ones do:
+ *      graphs of one engine run one at a time, on its stream ----------------------------------------- */
 /* RST_ACT_GELU: z (1 + erf(z / sqrt 2)) / 2;  RST_ACT_GELU_TANH: z (1 + tanh(sqrt(2 / pi) (z +
  * 0.044715 z^3))) / 2;  RST_ACT_SILU: z / (1 + exp(-z)).  At an infinite z all of them take their
  * limit (value 0 or z, derivative 0 or 1); NaN stays NaN, but RST_ACT_RELU takes it to 0, with derivative
@@ -172,7 +173,8 @@ int rst_activation_backward(rst_engine* engine, const double* grad, const double
 
 /* z = x[batch,in] . weight[out,in]^T + bias[1,out];  out[batch,out] = act(z) + residual[batch,out].
  * bias, residual: NULL for none.  pre_out[batch,out] receives z for the backward pass (NULL: not kept).
- * out may be residual itself; out and pre_out are no other operand (RST_ERR_INVALID_ARGUMENT). */
+ * out may be residual itself; otherwise out and pre_out share no element with an operand or each other
+ * (RST_ERR_INVALID_ARGUMENT). */
 int rst_linear_act_forward(rst_engine* engine, const double* x, const double* weight,
                            const double* bias, const double* residual, double* pre_out, double* out,
                            size_t batch, size_t in_features, size_t out_features, int activation);
@@ -184,9 +186,11 @@ int rst_linear_act_forward(rst_engine* engine, const double* x, const double* we
  * input_activation is what produced x from input_pre[batch,in] (its backward pass, fused as
  * rst_linear_backward fuses ReLU's; RST_ACT_NONE: input_pre is not used) and residual_grad[batch,in],
  * NULL for none, is what reaches this layer's input past it.  With both, residual_grad is the gradient
- * with respect to input_pre.  grad_input may be input_pre or residual_grad itself, but not what both
- * products read (x, weight, dz; RST_ERR_INVALID_ARGUMENT): a layer whose residual_grad is its grad
- * works in place where dz lies apart from both. */
+ * with respect to input_pre.  In place: grad_input may be input_pre or residual_grad itself, grad_pre as
+ * above.  Otherwise no output shares an element with what is read after it, or beside it, is written
+ * (RST_ERR_INVALID_ARGUMENT): grad_pre with x, weight, input_pre, residual_grad; grad_weight, grad_bias and
+ * grad_input with these, dz and each other.  So a layer whose residual_grad is its grad needs dz apart from it
+ * (grad_pre over pre, say), and then works in place; grad and pre themselves are free once dz is there. */
 int rst_linear_act_backward(rst_engine* engine, const double* grad, const double* pre, int activation,
                             double* grad_pre, const double* x, const double* weight,
                             double* grad_weight, double* grad_bias, double* grad_input,

@@ -3,6 +3,8 @@
 // conventions (division by the batch, gradients overwritten) are those of src/module/linear.rs:43-69.
 #include <climits>
 #include <cmath>
+#include <cstdint>
+#include <initializer_list>
 
 #include "common.h"
 
@@ -27,6 +29,26 @@ int check_probability(const char* who, double p) {
   if (!(p >= 0.0 && p < 1.0)) return fail(RST_ERR_INVALID_ARGUMENT, "%s: p = %g is not in [0, 1)", who, p);
   return RST_OK;
 }
+
+// An array of an entry point; count 0: not read or written in this call.
+struct Range {
+  const double* first;
+  size_t count;
+};
+bool overlap(const Range& a, const Range& b) {
+  if (!a.first || !b.first || a.count == 0 || b.count == 0) return false;
+  // (in doubles: a byte count of the largest extents does not fit)
+  const uintptr_t i = reinterpret_cast<uintptr_t>(a.first) / 8, j = reinterpret_cast<uintptr_t>(b.first) / 8;
+  return i < j + b.count && j < i + a.count;
+}
+// An output over something that workgroups still read or write while it is written.
+bool overlap_any(const Range& out, std::initializer_list<Range> others) {
+  for (const Range& other : others)
+    if (overlap(out, other)) return true;
+  return false;
+}
+// ... over an array that each element is read from just before it is written to: that array itself is fine
+bool overlap_shifted(const Range& out, const Range& in) { return out.first != in.first && overlap(out, in); }
 
 }  // namespace
 
@@ -99,14 +121,19 @@ int rst_linear_act_forward(rst_engine* e, const double* x, const double* weight,
   if (batch == 0 || out_features == 0) return RST_OK;
   if (!out || (in_features && (!x || !weight)))
     return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_forward: null operand");
-  // (other workgroups still read these)
-  if (out == x || out == weight || (pre_out && (pre_out == x || pre_out == weight || pre_out == residual || pre_out == out)))
-    return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_forward: an output over an operand");
   RST_TRY(check_dim("linear_act_forward", batch, "batch"));
   RST_TRY(check_dim("linear_act_forward", in_features, "in_features"));
   RST_TRY(check_dim("linear_act_forward", out_features, "out_features"));
+  const bool few_rows = linear_rows_supported(batch, out_features, in_features);
+  if (!few_rows) RST_TRY(check_contraction(batch, out_features));
+  {
+    const Range rx{x, batch * in_features}, rw{weight, out_features * in_features}, rb{bias, out_features};
+    const Range rr{residual, batch * out_features}, rp{pre_out, batch * out_features}, ro{out, batch * out_features};
+    if (overlap_any(ro, {rx, rw, rb, rp}) || overlap_shifted(ro, rr) || overlap_any(rp, {rx, rw, rb, rr}))
+      return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_forward: an output over an operand");
+  }
   const ActEpilogue act{activation, nullptr, residual, pre_out};
-  if (linear_rows_supported(batch, out_features, in_features))
+  if (few_rows)
     return launch_linear_rows(e->stream, x, weight, bias, out, act, batch, out_features, in_features);
   GemmDesc d{};
   d.A = x; d.B = weight; d.C = out;
@@ -136,14 +163,28 @@ int rst_linear_act_backward(rst_engine* e, const double* grad, const double* pre
     return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_backward: an activation needs pre and grad_pre");
   if (grad_input && input_activation != RST_ACT_NONE && !input_pre)
     return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_backward: an input activation needs input_pre");
-  // (both products read these while the input gradient is written)
-  if (grad_input && (grad_input == x || grad_input == weight || grad_input == (activation != RST_ACT_NONE ? grad_pre : grad)))
-    return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_backward: grad_input over x, weight or the products' gradient");
   RST_TRY(check_dim("linear_act_backward", batch, "batch"));
   RST_TRY(check_dim("linear_act_backward", in_features, "in_features"));
   RST_TRY(check_dim("linear_act_backward", out_features, "out_features"));
   RST_TRY(check_contraction(out_features, in_features));
   if (grad_input) RST_TRY(check_contraction(batch, in_features));
+  {
+    // what this call reads and writes: grad and pre are read before the products begin, and are free then; the input
+    // gradient, while the other gradients are written, reads what both products read, input_pre and residual_grad
+    const size_t above = batch * out_features, below = batch * in_features;
+    const bool act = activation != RST_ACT_NONE;
+    const Range rg{grad, above}, rpre{pre, act ? above : 0}, rdz{act ? grad_pre : grad, above};
+    const Range rx{x, below}, rw{weight, grad_input ? in_features * out_features : 0};
+    const Range rip{input_pre, grad_input && input_activation != RST_ACT_NONE ? below : 0};
+    const Range rres{residual_grad, grad_input ? below : 0};
+    const Range ow{grad_weight, in_features * out_features}, ob{grad_bias, out_features}, oi{grad_input, below};
+    if (act && (overlap_shifted(rdz, rg) || overlap_shifted(rdz, rpre) || overlap_any(rdz, {rx, rw, rip, rres})))
+      return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_backward: grad_pre over what is read after it is written");
+    if (overlap_any(ow, {rx, rw, rdz, rip, rres, ob, oi}) || overlap_any(ob, {rx, rw, rdz, rip, rres, oi}))
+      return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_backward: a parameter's gradient over another operand");
+    if (overlap_any(oi, {rx, rw, rdz}) || overlap_shifted(oi, rip) || overlap_shifted(oi, rres))
+      return fail(RST_ERR_INVALID_ARGUMENT, "linear_act_backward: grad_input over x, weight or the products' gradient");
+  }
   if (activation != RST_ACT_NONE) {
     RST_TRY(launch_act_backward(e->stream, activation, grad, pre, nullptr, grad_pre, batch * out_features));
     grad = grad_pre;

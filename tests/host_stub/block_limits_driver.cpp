@@ -42,7 +42,7 @@ extern "C" long hip_stub_launch_count();
 
 static rst_engine* e;
 // Operands that lie apart at any size (never dereferenced: kernels do not run)
-static double* at(int i) { return reinterpret_cast<double*>((uintptr_t)(i + 1) << 44); }
+static double* at(int i) { return reinterpret_cast<double*>((uintptr_t)(i + 1) << 59); }
 
 static int linear(size_t batch, size_t in, size_t out) {
   return rst_linear_act_forward(e, at(0), at(1), at(2), at(3), at(4), at(5), batch, in, out, RST_ACT_SILU);
@@ -70,7 +70,6 @@ int main() {
     LAUNCHES(linear(batch, 1, 100000000), 3);
     LAUNCHES(linear(batch, 1, most), 64);
     LAUNCHES(linear(batch, most, 1), 1);
-    LAUNCHES(linear(batch, most, most), 64);
   }
   // products: fewer than 2^23 tiles of 128x128, which is 2^30 - 128 of one extent while the other fits a tile
   const size_t last = ((size_t)1 << 30) - 128;

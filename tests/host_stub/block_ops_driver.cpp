@@ -45,6 +45,9 @@ int main() {
   EXPECT(rst_engine_create(0, &e), RST_OK);
   double* const p = reinterpret_cast<double*>((uintptr_t)1 << 40);  // never dereferenced: kernels do not run
   double *const q = p + ((size_t)1 << 36), *const r = q + ((size_t)1 << 36);
+  // (of an accepted backward pass: outputs that are no operand)
+  double *const x = r + ((size_t)1 << 36), *const w = x + ((size_t)1 << 36), *const gw = w + ((size_t)1 << 36);
+  double *const gb = gw + ((size_t)1 << 36), *const ip = gb + ((size_t)1 << 36), *const res = ip + ((size_t)1 << 36);
   double* const none = nullptr;
   const double nan = std::nan(""), inf = std::numeric_limits<double>::infinity();
   const size_t huge = (size_t)1 << 31;
@@ -148,14 +151,14 @@ int main() {
     EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, p, p, q, p, RST_ACT_GELU, p, zero == 0 ? 0 : 8,
                                    zero == 1 ? 0 : 8, zero == 2 ? 0 : 8), SHAPE);
   EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, p, p, q, p, RST_ACT_GELU, p, huge, 8, 8), UNSUPPORTED);
-  EXPECT(rst_linear_act_backward(e, p, none, RST_ACT_NONE, none, p, p, p, none, none, none, RST_ACT_GELU, none, 8, 8, 8), RST_OK);
+  EXPECT(rst_linear_act_backward(e, p, none, RST_ACT_NONE, none, p, p, gw, none, none, none, RST_ACT_GELU, none, 8, 8, 8), RST_OK);
   // grad_input over x, the weight, or the gradient that both products read
   EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, q, p, p, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
   EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, q, p, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
   EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, q, p, p, p, p, q, p, RST_ACT_GELU, p, 8, 8, 8), INVALID);
   EXPECT(rst_linear_act_backward(e, q, p, RST_ACT_GELU, q, p, p, p, p, q, p, RST_ACT_GELU, q, 8, 8, 8), INVALID);
   EXPECT(rst_linear_act_backward(e, q, none, RST_ACT_NONE, none, p, p, p, p, q, none, RST_ACT_NONE, q, 8, 8, 8), INVALID);
-  EXPECT(rst_linear_act_backward(e, q, p, RST_ACT_GELU, p, p, p, p, p, q, p, RST_ACT_GELU, q, 8, 8, 8), RST_OK);
+  EXPECT(rst_linear_act_backward(e, q, p, RST_ACT_GELU, p, x, w, gw, gb, q, ip, RST_ACT_GELU, q, 8, 8, 8), RST_OK);
 
   // inside a stream capture, over the routes of the planner
   const long allocations = hip_stub_allocation_calls();
@@ -165,12 +168,12 @@ int main() {
       for (size_t n : {1u, 10u, 101u, 1024u, 4608u})
         for (int act = RST_ACT_NONE; act <= RST_ACT_SILU; ++act) {
           EXPECT(rst_linear_act_forward(e, p, p, p, act & 1 ? p : none, act & 2 ? r : none, q, b, k, n, act), RST_OK);
-          EXPECT(rst_linear_act_backward(e, p, p, act, p, p, p, p, p, q, p, RST_ACT_SILU - act, act & 1 ? p : none, b, k, n), RST_OK);
+          EXPECT(rst_linear_act_backward(e, p, p, act, p, x, w, gw, gb, q, ip, RST_ACT_SILU - act, act & 1 ? res : none, b, k, n), RST_OK);
         }
   // slices of one gradient, of the other, of both, in the shared grid
   const size_t shared[][3] = {{1157, 233, 203}, {46, 2607, 939}, {518, 3, 2177}, {1953, 32, 3607}, {314, 1467, 790}, {2500, 20, 20}};
   for (auto& d : shared)
-    EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, p, p, p, p, q, p, RST_ACT_GELU, p, d[0], d[1], d[2]), RST_OK);
+    EXPECT(rst_linear_act_backward(e, p, p, RST_ACT_GELU, p, x, w, gw, gb, q, ip, RST_ACT_GELU, res, d[0], d[1], d[2]), RST_OK);
   EXPECT(rst_layer_norm_forward(e, p, p, p, p, p, p, 100, 1000, 1e-5), RST_OK);
   EXPECT(rst_layer_norm_backward(e, p, p, p, p, p, p, p, p, p, 100, 1000), RST_OK);
   EXPECT(rst_dropout_forward(e, p, p, p, 100, 0.5, 1, 2), RST_OK);
