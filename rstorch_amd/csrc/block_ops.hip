@@ -1,7 +1,6 @@
 // Operator-level C ABI of the residual block: layer norm, dropout, activations and the Linear layer
 // with activation and residual.  Argument checking and dispatch; the reference has no counterpart, the
 // conventions (division by the batch, gradients overwritten) are those of src/module/linear.rs:43-69.
-#include <climits>
 #include <cmath>
 #include <cstdint>
 #include <initializer_list>
@@ -12,8 +11,6 @@ using namespace rst;
 
 namespace {
 
-// (the last tile's row and column numbers are ints too)
-constexpr size_t kMostExtent = (size_t)INT_MAX - 127;
 int check_dim(const char* who, size_t v, const char* what) {
   if (v > kMostExtent) return fail(RST_ERR_UNSUPPORTED, "%s: %s = %zu exceeds 2^31-128", who, what, v);
   return RST_OK;

@@ -82,6 +82,9 @@ struct ActEpilogue {
   double* pre;             // forward: receives z, or NULL
 };
 
+// The largest extent of a product: row, column and contraction numbers are ints, those of the last tile's end as well.
+constexpr size_t kMostExtent = ((size_t)1 << 31) - 128;
+
 int launch_gemm(hipStream_t stream, const GemmDesc& d);
 // RST_ERR_UNSUPPORTED where launch_gemm would refuse a rows x cols result (2^23 tiles of 128x128 and more): what an
 // entry point of several launches asks before the first of them

@@ -8,7 +8,6 @@
 //             (input > 0) in the contraction epilogue, which is that ReLU's backward
 //             ([relu(z) > 0] == [z > 0], NaN included, both false);
 //   any ReLU not adjacent to a Linear runs the streaming kernels instead.
-#include <climits>
 #include <cstdlib>
 #include <cstring>
 #include <new>
@@ -250,7 +249,7 @@ struct Tail {
 // tail: its layers' inputs are noted, nothing is launched for them.
 int do_forward(rst_model* m, const double* x, size_t batch, double* final_out = nullptr, Tail tail = Tail()) {
   rst_engine* e = m->engine;
-  if (batch > (size_t)INT_MAX) return fail(RST_ERR_UNSUPPORTED, "batch too large");
+  if (batch > kMostExtent) return fail(RST_ERR_UNSUPPORTED, "batch too large");
   RST_TRY(reserve_activations(m, batch));
   m->batch = batch;
   const double* cur = x;
@@ -664,7 +663,7 @@ int rst_model_create(rst_engine* e, const int* kinds, const size_t* in_features,
       if (!in_features || !out_features) { delete m; return fail(RST_ERR_INVALID_ARGUMENT, "feature arrays are null"); }
       l.in = in_features[i];
       l.out = out_features[i];
-      if (l.in > (size_t)INT_MAX || l.out > (size_t)INT_MAX) { delete m; return fail(RST_ERR_UNSUPPORTED, "layer too wide"); }
+      if (l.in > kMostExtent || l.out > kMostExtent) { delete m; return fail(RST_ERR_UNSUPPORTED, "layer too wide"); }
       if (width_known && width != l.in) {
         int status = fail(RST_ERR_SHAPE, "layer %zu expects %zu inputs but receives %zu", i, l.in, width);
         delete m;

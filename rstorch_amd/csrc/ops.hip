@@ -1,6 +1,5 @@
 // Operator-level C ABI: argument checking and dispatch onto the launch functions.  Each entry
 // point names the reference lines it replaces in include/rstorch_hip.h.
-#include <climits>
 #include <cstring>
 
 #include "common.h"
@@ -34,7 +33,7 @@ namespace {
 __global__ void reset_softmax_flag_kernel(int* flags) { flags[2] = 0; }
 
 int check_dim(size_t v, const char* what) {
-  if (v > (size_t)INT_MAX) return fail(RST_ERR_UNSUPPORTED, "%s = %zu exceeds 2^31-1", what, v);
+  if (v > kMostExtent) return fail(RST_ERR_UNSUPPORTED, "%s = %zu exceeds 2^31-128", what, v);
   return RST_OK;
 }
 

@@ -108,9 +108,12 @@ int main() {
     REFUSED(backward(1, most, batch));
     REFUSED(backward(1, batch, most));
     LAUNCHES(linear(batch, most, 1), 2);
+    LAUNCHES(rst_linear_forward(e, at(0), at(1), at(2), at(5), batch, most, 1, 0), 2);
     for (size_t extent : {(size_t)INT_MAX - 1, (size_t)INT_MAX}) {
       REFUSED(rst_linear_forward(e, at(0), at(1), at(2), at(5), batch, 1, extent, 0));
       REFUSED(rst_linear_forward(e, at(0), at(1), at(2), at(5), extent, 1, batch, 0));
+      REFUSED(rst_linear_forward(e, at(0), at(1), at(2), at(5), batch, extent, 1, 0));
+      REFUSED(plain_backward(extent, batch, 1, false));
       REFUSED(plain_backward(extent, batch, 1));
       REFUSED(plain_backward(1, batch, extent));
     }
