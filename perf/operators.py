@@ -107,7 +107,18 @@ def draw(rng):
 
 
 # ---- inputs --------------------------------------------------------------------------------------
+def _share_stream():
+    """The engine works on a stream of its own, which torch's default one does not wait for, nor it for that.  A program
+    that hands torch's buffers to the engine lets torch work on the engine's stream: inputs are there before a call reads
+    them, and what torch does with the outputs comes after it."""
+    import rstorch_amd as rs
+    engine = rs.default_engine()
+    torch.cuda.set_stream(torch.cuda.ExternalStream(engine.lib.rst_engine_stream(engine.handle)))
+
+
 def prepare(case, seed):
+    if own:
+        _share_stream()
     g = torch.Generator(device=DEVICE)
     g.manual_seed(seed)
 
