@@ -48,7 +48,7 @@ PEAK_HBM_GBPS = 8000.0
 # the profile is collected again and the digest updated.
 C4_TRAFFIC_SOURCE = {"profile": "profiles/c4_hbm_traffic.md",
                      "kernel_sources": ["rstorch_amd/csrc/gemm_f64.hip", "rstorch_amd/csrc/gemm_addressing.h"],
-                     "kernel_sources_sha16": "a58eec86851cf2d2"}
+                     "kernel_sources_sha16": "894733154e7da907"}
 
 
 def kernel_sources_digest():
@@ -61,12 +61,12 @@ def kernel_sources_digest():
 
 
 C4_TRAFFIC_BYTES_PER_LAUNCH = {
-    "linear_forward": (8 * 436.5e6 + 3889.4e6) / 9,
-    "grad_weight": (8 * 862.4e6 + 7697.4e6) / 9,
-    "grad_input": (7 * 470.0e6 + 3335.3e6 + 134.3e6) / 8,
+    "linear_forward": (8 * 436.6e6 + 3823.4e6) / 9,
+    "grad_weight": (8 * 862.7e6 + 7479.2e6) / 9,
+    "grad_input": (7 * 470.0e6 + 3331.3e6 + 134.3e6) / 8,
     # a layer's weight gradient + SGD and the next layer's input gradient in one grid (the default):
     # six pairs at the hidden width and the one that carries the head's weight gradient
-    "grad_pair": (6 * 1526.1e6 + 8210.6e6) / 7,
+    "grad_pair": (6 * 1523.2e6 + 7949.0e6) / 7,
 }
 
 C4_SPEC = [("linear", 4096, 4096), ("relu",)] * 8 + [("linear", 4096, 32768)]

@@ -1159,8 +1159,9 @@ __global__ __launch_bounds__(WGM * WGN * 64, (BURST > 0 ? 1 : WGM * WGN >= 8 ? 4
 
 // A layer's weight gradient (p[0], the first workgroups) and its input gradient with the epilogue (p[1]) in one grid.
 // Bound by the trip to memory while a workgroup has a CU to itself (784 -> 100 features at 32 rows: 5.6 us), above by what the
-// tiles draw from L2, 8 TB/s at four flops a byte (1959 -> 388 at 734 rows: 69 us, 32 TFLOP/s).  64x64 tiles in this grid
-// draw half of that but are too few: 14 % faster to 45 % slower on 56 layers; two to six K steps at a time are level.
+// tiles draw from L2, 8 TB/s at four flops a byte (1959 -> 388 at 734 rows: 69 us, 32 TFLOP/s).  Register-staged 64x64
+// tiles in this grid draw half of that but are too few: 14 % faster to 45 % slower on 56 layers; two to six K steps at a time
+// are level.
 struct GradsPair {
   int first_block, first_reduce_block;  // of the input gradient
   GemmParams p[2];
