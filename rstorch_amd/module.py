@@ -838,21 +838,22 @@ class Residual(Module):
             self.inner = inner
         else:
             self.inner = Sequential(list(inner) if isinstance(inner, (list, tuple)) else [inner])
-        self._kept = None  # (shape, engine) of the last forward's input
+        self._kept = None  # (shape of the last forward's input, engine for the gradient)
 
     @classmethod
     def new(cls, inner):
         return cls(inner)
 
     def forward(self, input):
-        x = as_array2(input, self.inner._engine())
+        engine = self.inner._engine()
+        x = as_array2(input, engine)
         self.inner._drop_plan()  # (a compiled form would add in a pass of its own)
         wide = self.inner._output_size(x.cols)
         if wide is not None and wide != x.cols:
             raise _ffi.ShapeError(_ffi.RST_ERR_SHAPE, "a residual of %d features around layers that return %d"
                                   % (x.cols, wide))
         out = self.inner._layers_forward(x, x)
-        self._kept = (x.shape, x.engine)
+        self._kept = (x.shape, engine or x.engine)
         return out
 
     def backward(self, gradient):

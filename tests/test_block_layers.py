@@ -193,6 +193,14 @@ def test_host_arrays_go_to_the_engine_of_the_layers(recorder, monkeypatch, first
         assert out.engine is recorder
         assert rs.as_array2(model.backward(x)).engine is recorder
     assert not other.taken()
+    if outer is rs.Residual:  # an array that another engine handed over: the gradient belongs to the layers' engine
+        given, seen = Recorder(), []
+        monkeypatch.setattr(recorder, "from_numpy", lambda host: seen.append(host.shape) or recorder.empty(*host.shape))
+        monkeypatch.setattr(given, "from_numpy", None)
+        model = outer([lin()])
+        model.forward(given.empty(4, 6))
+        model.backward(x)
+        assert seen == [x.shape]
     # layers that are bound to no engine keep using the default one
     assert outer([rs.GELU(), rs.Dropout(0.5)]).forward(x).engine is other
 
